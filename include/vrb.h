@@ -325,6 +325,67 @@ int vrb_group_norm_apply_scatter(const void* x, int dtype, const void* weight, i
                                  int64_t spatial_full, int64_t spatial_offset, int groups,
                                  const float* mean, const float* inverse, int fuse_silu, vrb_stream stream);
 
+/* GroupNorm of a channels-last feature map, optionally followed by an activation: x and out are
+ * [batch, spatial, channels], statistics per (batch entry, group of channels / groups channels):
+ *   out = act((x - mean) * rsqrt(var + eps) * weight[c] + bias[c]),   one rounding, to x's dtype.
+ * The reference has no channels-last form; it would permute, call group_norm (:4919-5008) and permute
+ * back.  Unlike vrb_group_norm + SiLU the normalised value is not rounded before the activation.
+ * activation: a vrb_activation_kind or VRB_NO_ACTIVATION.  weight / bias (F32 or BF16, [channels]) may be
+ * NULL and are used as stored.  out may be x.  Results do not depend on the launch's timing.
+ * workspace: vrb_group_norm_channels_last_workspace_bytes() bytes of device scratch, 256-byte aligned
+ * (0 bytes: NULL is accepted); calls that may overlap on the GPU need scratch of their own. */
+#define VRB_NO_ACTIVATION (-1)
+size_t vrb_group_norm_channels_last_workspace_bytes(int dtype, int64_t batch, int64_t spatial, int64_t channels, int groups);
+int vrb_group_norm_channels_last(const void* x, int dtype, const void* weight, int weight_dtype,
+                                 const void* bias, int bias_dtype, void* out,
+                                 int64_t batch, int64_t spatial, int64_t channels, int groups, float eps,
+                                 int activation, void* workspace, size_t workspace_bytes, vrb_stream stream);
+
+/* ---- microscaled 4-bit floating point ----------------------------------------------------------
+ * Elements are OCP e2m1 codes (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign bit), blocks of consecutive elements of a
+ * row share a scale:
+ *   VRB_NVFP4  blocks of 16, scale e4m3, and one F32 scale per tensor: value = tensor_scale * scale * element
+ *   VRB_MXFP4  blocks of 32, scale 2^(byte - 127) (e8m0), no tensor scale (NULL): value = scale * element
+ * A packed operand [rows, k] is
+ *   codes   [rows, vrb_fp4_row_bytes(k)]: two elements to a byte, the even k in the low nibble, rows padded with
+ *           zeros to a multiple of 32 elements; 16-byte aligned
+ *   scales  vrb_fp4_scale_bytes(format, rows, k) bytes, 16-byte aligned, in the order the tensor core takes
+ *           them: tiles of 128 rows x 4 blocks of 512 bytes, block tiles innermost; the scale of (row, block) is byte
+ *           ((row / 128) * ceil(blocks / 4) + block / 4) * 512 + (row % 32) * 16 + (row % 128) / 32 * 4 + block % 4;
+ *           padding bytes are zero
+ * Weights are packed once and kept; activations are packed per call.  The reference stores weights in 8 bits or as
+ * integers (QuantType, native/include/vrhino/tensor.h:35) and has no 4-bit floating point. */
+typedef enum vrb_fp4_format { VRB_NVFP4 = 0, VRB_MXFP4 = 1 } vrb_fp4_format;
+int64_t vrb_fp4_row_bytes(int64_t k);
+size_t vrb_fp4_scale_bytes(int format, int64_t rows, int64_t k);
+
+/* tensor_scale[0] = max(|x|) / 2688 rounded to F32 (2688 = 6 * 448, the largest element times the largest block
+ * scale): the NVFP4 tensor scale that uses the whole range.  0 for a tensor of zeros; NaN if x holds a NaN. */
+int vrb_fp4_tensor_scale(const void* x, int dtype, int64_t count, float* tensor_scale, vrb_stream stream);
+
+/* Packs x [rows, k].  NVFP4: scale = e4m3(min(amax / (6 tensor_scale), 448)), element = e2m1(x / (tensor_scale *
+ * scale)); MXFP4: scale = 2^max(floor(log2 amax) - 2, -127), element = e2m1(x / scale), with amax the block's
+ * largest magnitude.  Both roundings are those of the exact quotients: to nearest, ties to the even code, saturating.
+ * tensor_scale: one F32 on the device (NULL = 1), finite and >= 0.  A block that holds an infinity or a NaN (or
+ * meets a tensor scale that is one) gets the NaN scale (0x7f / 0xff) and zero elements. */
+int vrb_fp4_quantize(int format, const void* x, int dtype, const float* tensor_scale, void* codes, void* scales,
+                     int64_t rows, int64_t k, vrb_stream stream);
+/* out [rows, k] = the values a packed operand stands for: tensor_scale * (scale * element), the inner product exact,
+ * the outer one in F32, then rounded to out_dtype. */
+int vrb_fp4_dequantize(int format, const void* codes, const void* scales, const float* tensor_scale, void* out,
+                       int out_dtype, int64_t rows, int64_t k, vrb_stream stream);
+
+/* The linear over two packed operands of one format, on the tensor cores that multiply block-scaled 4-bit elements:
+ *   out[m, n] = act(a_tensor_scale * b_tensor_scale * sum_k a[m, k] b[n, k] + bias[n])      [rows_a, rows_b]
+ * accumulated in F32, one rounding to out_dtype.  bias (F32 or BF16, [rows_b]) may be NULL; activation: a
+ * vrb_activation_kind or VRB_NO_ACTIVATION.  With F32 output, no bias and no activation the result is the accumulation
+ * that vrb_linear_output and its merged forms read.  Replaces a dequantisation (vrb_dequantize) and CudaBackend::linear
+ * (:3661-3866) where the weight is kept in 4 bits.  Needs the driver's cuTensorMapEncodeTiled (VRB_ERR_UNSUPPORTED
+ * otherwise).  Every wait inside is bounded; vrb_async_wait_failures reports one that ran out. */
+int vrb_fp4_linear(int format, const void* a_codes, const void* a_scales, const float* a_tensor_scale, int64_t rows_a,
+                   const void* b_codes, const void* b_scales, const float* b_tensor_scale, int64_t rows_b, int64_t k,
+                   const void* bias, int bias_dtype, int activation, void* out, int out_dtype, vrb_stream stream);
+
 /* ------------------------------------------------------------------------ fused chains -- */
 /* Each fused form produces what the cited chain of separate reference kernels produces,
  * including every intermediate rounding, while reading each tensor once. */

@@ -16,6 +16,8 @@ F32, BF16, U8 = 0, 2, 5
 SILU, GELU, GELU_TANH, TANH, RELU = 0, 1, 2, 3, 4
 ADD, MUL, DIV, MAX = 0, 1, 2, 3
 Q_FP8, Q_INT8, Q_INT4 = 0, 1, 2
+NVFP4, MXFP4 = 0, 1
+NO_ACTIVATION = -1
 
 
 class VrbError(RuntimeError):
@@ -54,6 +56,14 @@ SIGNATURES = {
     "vrb_group_norm_finalize": [_vp, _vp, _i64, _f, _vp, _vp, _vp],
     "vrb_group_norm_apply": [_vp, _i, _vp, _i, _vp, _i, _vp, _i64, _i64, _i64, _i, _vp, _vp, _i, _vp],
     "vrb_group_norm_apply_scatter": [_vp, _i, _vp, _i, _vp, _i, _vp, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i, _vp, _vp, _i, _vp],
+    "vrb_group_norm_channels_last_workspace_bytes": [_i, _i64, _i64, _i64, _i],
+    "vrb_group_norm_channels_last": [_vp, _i, _vp, _i, _vp, _i, _vp, _i64, _i64, _i64, _i, _f, _i, _vp, _sz, _vp],
+    "vrb_fp4_row_bytes": [_i64],
+    "vrb_fp4_scale_bytes": [_i, _i64, _i64],
+    "vrb_fp4_tensor_scale": [_vp, _i, _i64, _vp, _vp],
+    "vrb_fp4_quantize": [_i, _vp, _i, _vp, _vp, _vp, _i64, _i64, _vp],
+    "vrb_fp4_dequantize": [_i, _vp, _vp, _vp, _vp, _i, _i64, _i64, _vp],
+    "vrb_fp4_linear": [_i, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _i, _i, _vp, _i, _vp],
     "vrb_layer_norm_modulate": [_vp, _i, _vp, _i, _vp, _i, _vp, _vp, _i, _i64, _i64, _vp, _i, _i64, _i64, _f, _vp],
     "vrb_gated_residual_rms_norm_modulate": [_vp, _i, _vp, _i, _vp, _i, _i64, _i64, _vp, _i, _vp, _vp, _i, _i64, _i64,
                                              _vp, _i, _i64, _i64, _f, _vp],
@@ -108,6 +118,9 @@ _RESTYPES = {
     "vrb_device_allocation_count": _c.c_uint64,
     "vrb_group_norm_workspace_bytes": _c.c_size_t,
     "vrb_group_norm_frames_workspace_bytes": _c.c_size_t,
+    "vrb_group_norm_channels_last_workspace_bytes": _c.c_size_t,
+    "vrb_fp4_row_bytes": _c.c_int64,
+    "vrb_fp4_scale_bytes": _c.c_size_t,
     "vrb_host_release": None,
 }
 

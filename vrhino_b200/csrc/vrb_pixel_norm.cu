@@ -20,6 +20,7 @@
 // normalise pass of the reference read it twice.  Two tile buffers: the next tile's copies are in
 // flight while the current tile is reduced and written.  P is chosen so that three CTAs fit on an SM.
 #include "vrb_common.cuh"
+#include "vrb_fp4.cuh"
 #include "vrb_tma.cuh"
 
 #include <mutex>
@@ -787,7 +788,10 @@ int pixel_norm_family(const void* x, int dtype, const void* scale, const void* s
 
 extern "C" int vrb_async_wait_failures(int* failures) {
     VRB_REQUIRE(failures, VRB_ERR_INVALID, "async_wait_failures: null result");
-    const cudaError_t e = cudaMemcpyFromSymbol(failures, g_async_wait_gave_up, sizeof(int));
+    int linear = 0;   // the waits of vrb_fp4_linear have a flag of their own
+    cudaError_t e = cudaMemcpyFromSymbol(failures, g_async_wait_gave_up, sizeof(int));
+    if (e == cudaSuccess) e = fp4_wait_failures(&linear);
+    if (e == cudaSuccess && linear != 0) *failures = linear;
     if (e != cudaSuccess) {
         set_error("CUDA error: %s (async_wait_failures)", cudaGetErrorString(e));
         return VRB_ERR_CUDA;

@@ -7,12 +7,8 @@ namespace vrb {
 
 std::atomic<int> g_tma_tiles{1};
 
-bool encode_tile_map(CUtensorMap* map, const void* base, int dtype, int64_t outer, int64_t channels, int64_t inner,
-                     int box_inner, int box_channels) {
-    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static Encode encode = [] {
+void* tensor_map_encoder() {
+    static void* const encoder = [] {
         void* entry = nullptr;
         cudaDriverEntryPointQueryResult status;
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &entry, cudaEnableDefault, &status) != cudaSuccess ||
@@ -20,8 +16,17 @@ bool encode_tile_map(CUtensorMap* map, const void* base, int dtype, int64_t oute
             cudaGetLastError();
             entry = nullptr;
         }
-        return reinterpret_cast<Encode>(entry);
+        return entry;
     }();
+    return encoder;
+}
+
+bool encode_tile_map(CUtensorMap* map, const void* base, int dtype, int64_t outer, int64_t channels, int64_t inner,
+                     int box_inner, int box_channels) {
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    const Encode encode = reinterpret_cast<Encode>(tensor_map_encoder());
     if (!encode || !is_float_dtype(dtype) || box_inner < 1 || box_inner > 256 || box_channels < 1 || box_channels > 256) return false;
     const cuuint64_t element = dtype_bytes(dtype);
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(channels), static_cast<cuuint64_t>(outer)};

@@ -10,6 +10,8 @@
 
 namespace vrb {
 
+// The driver's cuTensorMapEncodeTiled, or nullptr where it offers none.
+void* tensor_map_encoder();
 // Encodes a rank-3 tiled map over x [outer, channels, inner] (innermost first: inner, channels, outer) with a box of
 // box_inner x box_channels x 1 elements, no swizzle, zero fill outside the tensor.  false: the driver entry point is
 // missing or refused the geometry (the caller then takes its cp.async path).

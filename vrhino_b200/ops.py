@@ -26,6 +26,7 @@ from ._lib import VrbError, call
 F32, BF16 = torch.float32, torch.bfloat16
 _CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.uint8: _lib.U8}
 SILU, GELU, GELU_TANH, TANH, RELU = 0, 1, 2, 3, 4
+NVFP4, MXFP4 = _lib.NVFP4, _lib.MXFP4
 
 
 def _ptr(t):
@@ -75,6 +76,28 @@ class RngState:
     seed: int = 0
     offset: int = 0
     algorithm_id: str = "pytorch_compat.v1"
+
+
+@dataclass
+class Fp4Tensor:
+    """A packed 4-bit operand [rows, k] (layout: include/vrb.h): codes [rows, row bytes] and scales are uint8 tensors,
+    tensor_scale is one F32 (NVFP4, None = 1) or None (MXFP4), shape the logical (..., k)."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    tensor_scale: torch.Tensor | None
+    format: int
+    shape: tuple
+
+    @property
+    def k(self):
+        return self.shape[-1]
+
+    @property
+    def rows(self):
+        rows = 1
+        for d in self.shape[:-1]:
+            rows *= d
+        return rows
 
 
 class HostScalar:
@@ -551,6 +574,95 @@ class B200Backend:
         call("vrb_group_norm_frames", _ptr(x), _code(x), _ptr(weight), _code(weight) if weight is not None else 0,
              _ptr(bias), _code(bias) if bias is not None else 0, _ptr(out), batch, channels, frames, spatial, groups,
              ctypes.c_float(eps), int(fuse_silu), _ptr(self._gn_workspace), need, _stream())
+        return out
+
+    def group_norm_channels_last(self, raw, groups, weight, bias, eps, activation=None, out=None):
+        """GroupNorm of [B, ..., C] with statistics per (batch entry, group of C / groups channels), then an optional
+        activation kind on the F32 value; one rounding to x's dtype.  The channels-last form of group_norm (which takes
+        [B, C, ...]), for feature maps whose rows the next linear reads."""
+        if raw.dim() < 2 or groups <= 0 or raw.shape[-1] % groups:
+            raise VrbError("group norm shape/groups mismatch")
+        weight, bias = self._param(weight), self._param(bias)
+        dtype = self._dtype_of(raw)
+        x = _dense(self.copy_to_device(raw, dtype))
+        batch, channels = x.shape[0], x.shape[-1]
+        for name, t in (("weight", weight), ("bias", bias)):
+            if t is not None and t.numel() != channels:
+                raise VrbError(f"group norm {name} mismatch")
+        out = _result(out, x.shape, x.dtype, x.device)
+        if x.numel() == 0:
+            return out
+        spatial = x.numel() // (batch * channels)
+        need = _lib.load().vrb_group_norm_channels_last_workspace_bytes(_code(x), batch, spatial, channels, groups)
+        # scratch of this call alone: torch's allocator keeps it from other streams and other captured graphs
+        scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+        call("vrb_group_norm_channels_last", _ptr(x), _code(x), _ptr(weight), _code(weight) if weight is not None else 0,
+             _ptr(bias), _code(bias) if bias is not None else 0, _ptr(out), batch, spatial, channels, groups,
+             ctypes.c_float(eps), _lib.NO_ACTIVATION if activation is None else int(activation), _ptr(scratch), need, _stream())
+        return out
+
+    # ---- microscaled 4-bit operands (include/vrb.h) ----
+    def fp4_tensor_scale(self, raw, out=None):
+        """The NVFP4 tensor scale of x as a device F32 [1]: max(|x|) / 2688."""
+        x = _dense(self.copy_to_device(raw, self._dtype_of(raw)))
+        out = _result(out, (1,), F32, x.device)
+        call("vrb_fp4_tensor_scale", _ptr(x), _code(x), x.numel(), _ptr(out), _stream())
+        return out
+
+    def fp4_quantize(self, raw, format=NVFP4, tensor_scale=None, out=None):
+        """Packs x [..., k] into 4 bits an element with a scale per block of a row; NVFP4 takes a device F32 tensor scale
+        (fp4_tensor_scale, or one calibrated beforehand; None = 1)."""
+        x = _dense(self.copy_to_device(raw, self._dtype_of(raw)))
+        if x.dim() < 1 or x.numel() == 0:
+            raise VrbError("fp4_quantize: rows and k must be positive")
+        k = x.shape[-1]
+        rows = x.numel() // k
+        lib = _lib.load()
+        code_shape, scale_bytes = (rows, lib.vrb_fp4_row_bytes(k)), lib.vrb_fp4_scale_bytes(format, rows, k)
+        if out is not None and (out.format != format or out.tensor_scale is not tensor_scale or tuple(out.shape) != tuple(x.shape)):
+            raise VrbError("output buffer does not match the result's shape, dtype or device")
+        codes = _result(None if out is None else out.codes, code_shape, torch.uint8, x.device)
+        scales = _result(None if out is None else out.scales, (scale_bytes,), torch.uint8, x.device)
+        self._fp4_scale(tensor_scale, x.device)
+        call("vrb_fp4_quantize", format, _ptr(x), _code(x), _ptr(tensor_scale), _ptr(codes), _ptr(scales), rows, k, _stream())
+        return out if out is not None else Fp4Tensor(codes, scales, tensor_scale, format, tuple(x.shape))
+
+    @staticmethod
+    def _fp4_scale(tensor_scale, device):
+        if tensor_scale is not None and (tensor_scale.dtype != F32 or tensor_scale.numel() != 1 or tensor_scale.device != device):
+            raise VrbError("fp4 tensor scale must be one F32 on the operand's device")
+
+    def _fp4_operand(self, q):
+        lib = _lib.load()
+        rows, k = q.rows, q.k
+        if rows <= 0 or k <= 0 or tuple(q.codes.shape) != (rows, lib.vrb_fp4_row_bytes(k)) or q.codes.dtype != torch.uint8 or \
+                q.scales.dtype != torch.uint8 or q.scales.numel() != lib.vrb_fp4_scale_bytes(q.format, rows, k):
+            raise VrbError("fp4 operand: codes or scales do not match the shape and format")
+        _dense(q.codes), _dense(q.scales)
+        self._fp4_scale(q.tensor_scale, q.codes.device)
+        return rows, k
+
+    def fp4_dequantize(self, q, dtype=BF16, out=None):
+        """The values a packed operand stands for, in `dtype` (the 4-bit sibling of dequantize)."""
+        rows, k = self._fp4_operand(q)
+        out = _result(out, q.shape, dtype, q.codes.device)
+        call("vrb_fp4_dequantize", q.format, _ptr(q.codes), _ptr(q.scales), _ptr(q.tensor_scale), _ptr(out), _code(dtype), rows, k, _stream())
+        return out
+
+    def fp4_linear(self, x, weight, bias=None, activation=None, dtype=BF16, out=None):
+        """activation(x weight^T + bias) over packed operands x [..., k] and weight [n, k] of one format -> [..., n] in
+        `dtype`, accumulated in F32.  dtype F32 without bias and activation is the accumulation that linear_output and
+        its merged forms read."""
+        m, k = self._fp4_operand(x)
+        n, kw = self._fp4_operand(weight)
+        if x.format != weight.format or k != kw or len(weight.shape) != 2:
+            raise VrbError("fp4_linear: operands differ in format or width")
+        if bias is not None and (_dense(bias).numel() != n):
+            raise VrbError("linear bias mismatch")
+        out = _result(out, tuple(x.shape[:-1]) + (n,), dtype, x.codes.device)
+        call("vrb_fp4_linear", x.format, _ptr(x.codes), _ptr(x.scales), _ptr(x.tensor_scale), m, _ptr(weight.codes), _ptr(weight.scales),
+             _ptr(weight.tensor_scale), n, k, _ptr(bias), _code(bias) if bias is not None else 0,
+             _lib.NO_ACTIVATION if activation is None else int(activation), _ptr(out), _code(dtype), _stream())
         return out
 
 
