@@ -615,6 +615,8 @@ class B200Backend:
         x = _dense(self.copy_to_device(raw, self._dtype_of(raw)))
         if x.dim() < 1 or x.numel() == 0:
             raise VrbError("fp4_quantize: rows and k must be positive")
+        if format not in (NVFP4, MXFP4):
+            raise VrbError(f"fp4_quantize: unknown 4-bit format {format}")
         k = x.shape[-1]
         rows = x.numel() // k
         lib = _lib.load()
