@@ -13,7 +13,7 @@
 //               buffer's scale columns are its own, so the buffer's barrier also guards them
 //   warps 2-9   take the accumulator out of tensor memory in one go (128 registers a thread: 256 accumulator columns and
 //               the scales leave no room for a second one), release it, and apply scale, bias and activation and
-//               write rows while the next tile's products run
+//               store boxes of 32 rows through shared memory while the next tile's products run
 // Every wait is bounded: one that runs out sets a flag that the host can read and ends the CTA.
 #include <cuda.h>
 
@@ -41,8 +41,7 @@ struct LinearArgs {
     int64_t m, n;
     int64_t k;
     int bias_dt, out_dt, activation;
-    int vector_out;            // bytes that rows of out are aligned to: 32, 16 or 0
-    int vector_bias;           // 8 bias values may be read at a time
+    int boxed;                 // rows of out lie on 16-byte boundaries: stored as boxes
 };
 
 __device__ __forceinline__ unsigned long long now_ns() {
@@ -158,78 +157,73 @@ __device__ __forceinline__ void tile_of(int64_t index, int64_t row_tiles, int64_
     row_tile = first + within - column_tile * height;
 }
 
-// SiLU and GELU-tanh through one exponential and one reciprocal: relative error below 2^-20, far under the bf16 step.
-// ACT: 0 none, 1 SiLU, 2 GELU-tanh, 3 any other kind
+// y sigmoid(w) for two values: SiLU (w = y) and GELU-tanh (w = 2 sqrt(2 / pi) (y + 0.044715 y^3)), as y / (1 + 2^z) with
+// z = -w log2(e).  The epilogue is bound by the special-function unit, so both share a reciprocal: 1 / (d0 d1), times the
+// other's d.  z is cut at 63 so that the product stays finite (the result is then below |y| 2^-63; a NaN's z becomes 63 and
+// the NaN returns with the factor y, without touching its neighbour).  Relative error below 2^-20, far under the bf16 step.
 template <int ACT>
-__device__ __forceinline__ float linear_activation(float y, int kind) {
-    if constexpr (ACT == 0) return y;
-    if constexpr (ACT == 1) return __fdividef(y, 1.0f + __expf(-y));
-    if constexpr (ACT == 2) {
-        const float u = 0.7978845608028654f * (y + 0.044715f * y * y * y);
-        return __fdividef(y, 1.0f + __expf(-2.0f * u));
-    }
-    return activation_value(kind, y);
+__device__ __forceinline__ void gate_pair(unsigned long long y, float& out0, float& out1) {
+    constexpr float kLog2E = 1.4426950408889634f, kGelu = -2.0f * 0.7978845608028654f * kLog2E;
+    unsigned long long z;
+    if constexpr (ACT == 1) z = mul_f32x2(y, pack_f32x2(-kLog2E, -kLog2E));
+    else z = mul_f32x2(y, fma_f32x2(mul_f32x2(y, y), pack_f32x2(0.044715f * kGelu, 0.044715f * kGelu), pack_f32x2(kGelu, kGelu)));
+    float z0, z1, e0, e1, d0, d1, y0, y1, r;
+    unpack_f32x2(z, z0, z1);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(fminf(z0, 63.0f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(fminf(z1, 63.0f)));
+    unpack_f32x2(add_f32x2(pack_f32x2(e0, e1), pack_f32x2(1.0f, 1.0f)), d0, d1);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d0 * d1));
+    unpack_f32x2(y, y0, y1);
+    out0 = y0 * (r * d1);
+    out1 = y1 * (r * d0);
 }
 
-// v[0 .. 32) = act(alpha * v + bias[column ..]): the product rounded to F32 before the bias is added, as the framework's
-// epilogue does with a stored accumulation
-template <int ACT>
-__device__ __forceinline__ void finish_columns(const LinearArgs& p, int64_t column, float alpha, float* v) {
+// ACT: 0 none, 1 SiLU, 2 GELU-tanh, 3 any other kind.  v[0 .. N) = act(alpha * v + bias): the product rounded to F32 before the
+// bias is added, as the framework's epilogue does with a stored accumulation.  bias: F32 in shared memory or nullptr.
+template <int ACT, int N>
+__device__ __forceinline__ void finish_columns(float* v, const float* bias, float alpha, int kind) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-        float b[8];
-        if (p.bias && p.vector_bias && column + i < p.n) {
-            load8<false>(p.bias, p.bias_dt, column + i, b);
+    for (int i = 0; i < N; i += 4) {
+        float4 b = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (bias) b = *reinterpret_cast<const float4*>(bias + i);
+        const unsigned long long lo = add_f32x2(pack_f32x2(__fmul_rn(v[i], alpha), __fmul_rn(v[i + 1], alpha)), pack_f32x2(b.x, b.y));
+        const unsigned long long hi = add_f32x2(pack_f32x2(__fmul_rn(v[i + 2], alpha), __fmul_rn(v[i + 3], alpha)), pack_f32x2(b.z, b.w));
+        if constexpr (ACT == 1 || ACT == 2) {
+            gate_pair<ACT>(lo, v[i], v[i + 1]);
+            gate_pair<ACT>(hi, v[i + 2], v[i + 3]);
         } else {
+            unpack_f32x2(lo, v[i], v[i + 1]);
+            unpack_f32x2(hi, v[i + 2], v[i + 3]);
+            if constexpr (ACT == 3)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) b[e] = p.bias && column + i + e < p.n ? load1(p.bias, p.bias_dt, column + i + e) : 0.0f;
+                for (int e = 0; e < 4; ++e) v[i + e] = activation_value(kind, v[i + e]);
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[i + e] = linear_activation<ACT>(__fadd_rn(__fmul_rn(v[i + e], alpha), b[e]), p.activation);
     }
 }
-// 32 columns of a row of the result, rows on vector boundaries
-__device__ __forceinline__ void store_columns(const LinearArgs& p, int64_t row, int64_t column, const float* v) {
-    const int64_t at = row * p.n + column;
-    if (p.out_dt == VRB_BF16) {
-        uint16_t* o = static_cast<uint16_t*>(p.out) + at;
+// 128 bytes of this lane's row into the warp's box of 32 rows (128-byte swizzle)
+__device__ __forceinline__ void stage_row(unsigned box, int lane, const uint32_t (&w)[32]) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 16) {
-            const uint4 lo = make_uint4(pack_bf16x2(v[i], v[i + 1]), pack_bf16x2(v[i + 2], v[i + 3]), pack_bf16x2(v[i + 4], v[i + 5]), pack_bf16x2(v[i + 6], v[i + 7]));
-            const uint4 hi = make_uint4(pack_bf16x2(v[i + 8], v[i + 9]), pack_bf16x2(v[i + 10], v[i + 11]), pack_bf16x2(v[i + 12], v[i + 13]), pack_bf16x2(v[i + 14], v[i + 15]));
-            if (p.vector_out == 32 && column + i < p.n) {
-                store32_aligned(o + i, lo, hi);
-            } else {
-                if (column + i < p.n) *reinterpret_cast<uint4*>(o + i) = lo;
-                if (column + i + 8 < p.n) *reinterpret_cast<uint4*>(o + i + 8) = hi;
-            }
-        }
-    } else {
-        float* o = static_cast<float*>(p.out) + at;
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-            const uint4 lo = make_uint4(__float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3]));
-            const uint4 hi = make_uint4(__float_as_uint(v[i + 4]), __float_as_uint(v[i + 5]), __float_as_uint(v[i + 6]), __float_as_uint(v[i + 7]));
-            if (p.vector_out == 32 && column + i < p.n) {
-                store32_aligned(o + i, lo, hi);
-            } else {
-                if (column + i < p.n) *reinterpret_cast<uint4*>(o + i) = lo;
-                if (column + i + 4 < p.n) *reinterpret_cast<uint4*>(o + i + 4) = hi;
-            }
-        }
-    }
+    for (int c = 0; c < 8; ++c)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + lane * 128 + ((c ^ (lane & 7)) << 4)), "r"(w[4 * c]), "r"(w[4 * c + 1]),
+                     "r"(w[4 * c + 2]), "r"(w[4 * c + 3])
+                     : "memory");
+}
+__device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int y, unsigned box) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(box)
+                 : "memory");
 }
 
 // ------------------------------------------------------------------------------------- pair kernel --
 constexpr int kPairThreads = 320;
 constexpr int kPairTile = 256;
-constexpr int kPairStages = 5;
+constexpr int kPairStages = 4;
 constexpr int kPairBufferBytes = 2 * kCodeBytes + 3 * kScaleBytes;   // a codes, b codes, a scales, b scales of all 256 columns
 constexpr int kPairColumns = 512;          // tensor memory: 256 accumulator columns, then 48 scale columns a buffer
 constexpr int kPairScaleColumns = 48;
-constexpr int kScratchRow = 33;            // floats; odd, so that a column of a warp's scratch hits 32 banks
-constexpr int kScratchBytes = 8 * 32 * kScratchRow * 4;
-constexpr int kPairSharedBytes = kPairStages * kPairBufferBytes + kScratchBytes + 1024;   // + alignment of the swizzled tiles
+constexpr int kBoxBytes = 32 * 128;        // 32 rows of 128 bytes of the result
+constexpr int kPairWriters = 8;
+// + alignment of the swizzled tiles; two boxes and 128 bias values a writing warp
+constexpr int kPairSharedBytes = kPairStages * kPairBufferBytes + kPairWriters * (2 * kBoxBytes + 512) + 1024;
 static_assert(kPairTile + kPairStages * kPairScaleColumns <= kPairColumns, "scales do not fit tensor memory");
 
 struct PairControl {
@@ -238,10 +232,11 @@ struct PairControl {
     volatile int abort;
 };
 
-template <int FORMAT, int ACT>
+template <int FORMAT, int ACT, int OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map,
-                       const __grid_constant__ CUtensorMap a_scale_map, const __grid_constant__ CUtensorMap b_scale_map, const LinearArgs p) {
+                       const __grid_constant__ CUtensorMap a_scale_map, const __grid_constant__ CUtensorMap b_scale_map,
+                       const __grid_constant__ CUtensorMap out_map, const LinearArgs p) {
     extern __shared__ uint8_t dynamic_shared[];
     __shared__ PairControl control;
     const unsigned buffers = (shared_address(dynamic_shared) + 1023u) & ~1023u;
@@ -341,13 +336,21 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
         const int quarter = warp & 3;                  // the 32 tensor-memory lanes this warp may read
         const int side = (warp - 2) >> 2;              // its half of the columns
         const float alpha = __fmul_rn(p.a_scale ? *p.a_scale : 1.0f, p.b_scale ? *p.b_scale : 1.0f);
-        float* scratch = reinterpret_cast<float*>(dynamic_shared + (buffers - shared_address(dynamic_shared)) + kPairStages * kPairBufferBytes) +
-                         (warp - 2) * 32 * kScratchRow;
+        const unsigned boxes = buffers + kPairStages * kPairBufferBytes + (warp - 2) * 2 * kBoxBytes;
+        uint8_t* generic = dynamic_shared + (buffers - shared_address(dynamic_shared)) + kPairStages * kPairBufferBytes;
+        float* scratch = reinterpret_cast<float*>(generic + (warp - 2) * 2 * kBoxBytes);
+        float* bias = reinterpret_cast<float*>(generic + kPairWriters * 2 * kBoxBytes) + (warp - 2) * 128;
+        int turn = 0;
         const unsigned drained = map_to_rank(shared_address(&control.drained), 0);
         unsigned phase = 0;
         for (int64_t t = pair; t < tiles; t += pairs) {
             int64_t row_tile, column_tile;
             tile_of(t, row_tiles, column_tiles, row_tile, column_tile);
+            const int64_t column0 = column_tile * kPairTile + side * 128;
+            if (p.bias) {   // before the wait: the loads are over when the accumulator is
+#pragma unroll
+                for (int c = 0; c < 128; c += 32) bias[c + lane] = column0 + c + lane < p.n ? load1(p.bias, p.bias_dt, column0 + c + lane) : 0.0f;
+            }
             if (!__all_sync(0xffffffffu, wait_barrier(&control.done, phase, &control.abort))) break;
             phase ^= 1u;
             fence_after();
@@ -359,26 +362,46 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
             fence_before();
             __syncwarp();
             if (lane == 0) arrive_cluster(drained);
-            const int64_t row0 = row_tile * kPairTile + rank * kRows + quarter * 32, row = row0 + lane;
+            const int64_t row0 = row_tile * kPairTile + rank * kRows + quarter * 32;
+            const float* tile_bias = p.bias ? bias : nullptr;
+            if (p.boxed) {
+                constexpr int N = OUT == VRB_BF16 ? 64 : 32;   // columns of a box
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int64_t column = column_tile * kPairTile + side * 128 + c * 32;
-                finish_columns<ACT>(p, column, alpha, v + c * 32);
-                if (p.vector_out) {
-                    if (row < p.m && column < p.n) store_columns(p, row, column, v + c * 32);
-                } else {
-                    // rows off the vector boundaries: through the warp's scratch, so that a store covers 32 columns of a row
+                for (int c = 0; c < 128; c += N) {
+                    finish_columns<ACT, N>(v + c, p.bias ? tile_bias + c : nullptr, alpha, p.activation);
+                    uint32_t w[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) w[i] = OUT == VRB_BF16 ? pack_bf16x2(v[c + 2 * i % N], v[c + (2 * i + 1) % N]) : __float_as_uint(v[c + i]);
+                    const unsigned box = boxes + turn * kBoxBytes;
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");   // the box's store before last has read it
+                    __syncwarp();
+                    stage_row(box, lane, w);
+                    async_proxy_fence();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (row0 < p.m && column0 + c < p.n) store_box(&out_map, static_cast<int>(column0 + c), static_cast<int>(row0), box);
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");   // an empty group too: the waits count them
+                    }
+                    turn ^= 1;
+                }
+            } else {
+                // rows off the 16-byte boundaries that a box needs: through scratch, so that a store covers 32 columns of a row
+                const int height = static_cast<int>(p.m - row0 < 32 ? p.m - row0 : 32);
+#pragma unroll
+                for (int c = 0; c < 128; c += 32) {
+                    finish_columns<ACT, 32>(v + c, p.bias ? tile_bias + c : nullptr, alpha, p.activation);
                     __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) scratch[lane * kScratchRow + i] = v[c * 32 + i];
+                    for (int i = 0; i < 32; ++i) scratch[lane * 32 + (i ^ lane)] = v[c + i];
                     __syncwarp();
-                    const int height = static_cast<int>(p.m - row0 < 32 ? p.m - row0 : 32);
-                    if (column + lane < p.n)
-                        for (int r = 0; r < height; ++r) store1(p.out, p.out_dt, (row0 + r) * p.n + column + lane, scratch[r * kScratchRow + lane]);
+                    const int64_t column = column0 + c + lane;
+                    if (column < p.n)
+                        for (int r = 0; r < height; ++r) store1(p.out, OUT, (row0 + r) * p.n + column, scratch[r * 32 + (lane ^ r)]);
                 }
             }
             __syncwarp();
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     __syncwarp();
     fence_before();
@@ -418,22 +441,26 @@ bool encode_scales(CUtensorMap* map, int format, const void* scales, int64_t row
                      CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-template <int FORMAT, int ACT>
-int launch_pair(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& sa, const CUtensorMap& sb, const LinearArgs& p, cudaStream_t s) {
+struct LinearMaps {
+    CUtensorMap a, b, a_scales, b_scales, out;
+};
+
+template <int FORMAT, int ACT, int OUT>
+int launch_pair(const LinearMaps& maps, const LinearArgs& p, cudaStream_t s) {
     static_assert(kPairSharedBytes + sizeof(PairControl) <= 227 * 1024, "ring does not fit shared memory");
-    const cudaError_t e = cudaFuncSetAttribute(fp4_linear_pair_kernel<FORMAT, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSharedBytes);
+    const cudaError_t e = cudaFuncSetAttribute(fp4_linear_pair_kernel<FORMAT, ACT, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSharedBytes);
     VRB_REQUIRE(e == cudaSuccess, VRB_ERR_CUDA, "CUDA error: %s (fp4_linear)", cudaGetErrorString(e));
     const int64_t tiles = ((p.m + kPairTile - 1) / kPairTile) * ((p.n + kPairTile - 1) / kPairTile), pairs = sm_count() / 2;
-    launch_overlapped(fp4_linear_pair_kernel<FORMAT, ACT>, dim3(static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs))), dim3(kPairThreads), kPairSharedBytes, s,
-                      a, b, sa, sb, p);
+    launch_overlapped(fp4_linear_pair_kernel<FORMAT, ACT, OUT>, dim3(static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs))), dim3(kPairThreads),
+                      kPairSharedBytes, s, maps.a, maps.b, maps.a_scales, maps.b_scales, maps.out, p);
     return after_launch("fp4_linear");
 }
-template <int FORMAT>
-int launch_linear(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& sa, const CUtensorMap& sb, const LinearArgs& p, cudaStream_t s) {
-    if (p.activation == VRB_NO_ACTIVATION) return launch_pair<FORMAT, 0>(a, b, sa, sb, p, s);
-    if (p.activation == VRB_SILU) return launch_pair<FORMAT, 1>(a, b, sa, sb, p, s);
-    if (p.activation == VRB_GELU_TANH) return launch_pair<FORMAT, 2>(a, b, sa, sb, p, s);
-    return launch_pair<FORMAT, 3>(a, b, sa, sb, p, s);
+template <int FORMAT, int OUT>
+int launch_linear(const LinearMaps& maps, const LinearArgs& p, cudaStream_t s) {
+    if (p.activation == VRB_NO_ACTIVATION) return launch_pair<FORMAT, 0, OUT>(maps, p, s);
+    if (p.activation == VRB_SILU) return launch_pair<FORMAT, 1, OUT>(maps, p, s);
+    if (p.activation == VRB_GELU_TANH) return launch_pair<FORMAT, 2, OUT>(maps, p, s);
+    return launch_pair<FORMAT, 3, OUT>(maps, p, s);
 }
 
 }  // namespace
@@ -460,14 +487,15 @@ extern "C" int vrb_fp4_linear(int format, const void* a_codes, const void* a_sca
     p.a_scale = a_tensor_scale; p.b_scale = b_tensor_scale;
     p.bias = bias; p.bias_dt = bias_dtype; p.out = out; p.out_dt = out_dtype; p.activation = activation;
     p.m = rows_a; p.n = rows_b; p.k = k;
-    // stores of 32 bytes need whole rows of them; 16 bytes likewise
-    const int64_t row_bytes = rows_b * static_cast<int64_t>(dtype_bytes(out_dtype));
-    const uintptr_t address = reinterpret_cast<uintptr_t>(out);
-    p.vector_out = row_bytes % 32 == 0 && address % 32 == 0 ? 32 : row_bytes % 16 == 0 && address % 16 == 0 ? 16 : 0;
-    p.vector_bias = bias && aligned16(bias) && rows_b % 8 == 0;
-    CUtensorMap a, b, sa, sb;
-    VRB_REQUIRE(encode_codes(&a, a_codes, rows_a, k, kRows) && encode_codes(&b, b_codes, rows_b, k, kRows) && encode_scales(&sa, format, a_scales, rows_a, k, 1) &&
-                    encode_scales(&sb, format, b_scales, rows_b, k, 2),
+    const int64_t element = static_cast<int64_t>(dtype_bytes(out_dtype));
+    p.boxed = aligned16(out) && rows_b * element % 16 == 0;
+    LinearMaps maps{};
+    VRB_REQUIRE(encode_codes(&maps.a, a_codes, rows_a, k, kRows) && encode_codes(&maps.b, b_codes, rows_b, k, kRows) &&
+                    encode_scales(&maps.a_scales, format, a_scales, rows_a, k, 1) && encode_scales(&maps.b_scales, format, b_scales, rows_b, k, 2) &&
+                    (!p.boxed || encode_2d(&maps.out, out_dtype == VRB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, out, rows_b,
+                                           rows_a, rows_b * element, static_cast<int>(128 / element), 32, CU_TENSOR_MAP_SWIZZLE_128B)),
                 VRB_ERR_UNSUPPORTED, "fp4_linear: the driver offers no tensor maps for these operands");
-    return format == VRB_NVFP4 ? launch_linear<VRB_NVFP4>(a, b, sa, sb, p, as_stream(stream)) : launch_linear<VRB_MXFP4>(a, b, sa, sb, p, as_stream(stream));
+    cudaStream_t s = as_stream(stream);
+    if (format == VRB_NVFP4) return out_dtype == VRB_BF16 ? launch_linear<VRB_NVFP4, VRB_BF16>(maps, p, s) : launch_linear<VRB_NVFP4, VRB_F32>(maps, p, s);
+    return out_dtype == VRB_BF16 ? launch_linear<VRB_MXFP4, VRB_BF16>(maps, p, s) : launch_linear<VRB_MXFP4, VRB_F32>(maps, p, s);
 }
