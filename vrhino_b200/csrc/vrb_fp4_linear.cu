@@ -11,7 +11,7 @@
 //               zeros outside the operand), scale tiles by a map of 8-byte words
 //   warp 1      of the pair's first CTA copies the scale tiles on into tensor memory and issues the products; a
 //               buffer's scale columns are its own, so the buffer's barrier also guards them
-//   warps 2-9   take the accumulator out of tensor memory in one go (128 registers a thread: 256 accumulator columns and
+//   warps 2-17  take the accumulator out of tensor memory in one go (64 registers a thread: 256 accumulator columns and
 //               the scales leave no room for a second one), release it, and apply scale, bias and activation and
 //               store boxes of 32 rows through shared memory while the next tile's products run
 // Every wait is bounded: one that runs out sets a flag that the host can read and ends the CTA.
@@ -49,14 +49,13 @@ __device__ __forceinline__ unsigned long long now_ns() {
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
     return t;
 }
-// Waits for the phase with the given parity; false: gave up (or another warp of the CTA did).  Acquires at cluster
-// scope: the arrival may come from the pair's other CTA.
+// Waits for the phase with the given parity; false: gave up (or another warp of the CTA did).
 __device__ __forceinline__ bool wait_barrier(uint64_t* barrier, unsigned parity, volatile int* abort) {
     const unsigned address = shared_address(barrier);
     unsigned long long start = 0;
     for (unsigned tries = 0;; ++tries) {
         unsigned done;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                      : "=r"(done) : "r"(address), "r"(parity) : "memory");
         if (done) return true;
         if ((tries & 63u) == 63u) {
@@ -84,8 +83,10 @@ __device__ __forceinline__ unsigned map_to_rank(unsigned address, unsigned rank)
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
+// Arrives on a barrier of either CTA.  CTA scope is enough: what it orders is tensor memory, by the tcgen05 fences around
+// it (a release at cluster scope waits for every earlier store of the warp, 1000 to 1800 cycles a tile).
 __device__ __forceinline__ void arrive_cluster(unsigned barrier_address) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(barrier_address) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(barrier_address) : "memory");
 }
 __device__ __forceinline__ bool elect_one() {
     unsigned r;
@@ -178,16 +179,23 @@ __device__ __forceinline__ void gate_pair(unsigned long long y, float& out0, flo
     out1 = y1 * (r * d0);
 }
 
-// ACT: 0 none, 1 SiLU, 2 GELU-tanh, 3 any other kind.  v[0 .. N) = act(alpha * v + bias): the product rounded to F32 before the
-// bias is added, as the framework's epilogue does with a stored accumulation.  bias: F32 in shared memory or nullptr.
+// ACT: 0 none, 1 SiLU, 2 GELU-tanh, 3 any other kind.  v[0 .. N) = act(alpha * v + bias); without an activation the product
+// is rounded to F32 before the bias is added, so that the result has the bits of vrb_linear_output on the stored
+// accumulation.  bias: F32 in shared memory or nullptr.
 template <int ACT, int N>
 __device__ __forceinline__ void finish_columns(float* v, const float* bias, float alpha, int kind) {
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
         float4 b = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (bias) b = *reinterpret_cast<const float4*>(bias + i);
-        const unsigned long long lo = add_f32x2(pack_f32x2(__fmul_rn(v[i], alpha), __fmul_rn(v[i + 1], alpha)), pack_f32x2(b.x, b.y));
-        const unsigned long long hi = add_f32x2(pack_f32x2(__fmul_rn(v[i + 2], alpha), __fmul_rn(v[i + 3], alpha)), pack_f32x2(b.z, b.w));
+        unsigned long long lo, hi;
+        if constexpr (ACT == 1 || ACT == 2) {
+            lo = fma_f32x2(pack_f32x2(v[i], v[i + 1]), pack_f32x2(alpha, alpha), pack_f32x2(b.x, b.y));
+            hi = fma_f32x2(pack_f32x2(v[i + 2], v[i + 3]), pack_f32x2(alpha, alpha), pack_f32x2(b.z, b.w));
+        } else {
+            lo = add_f32x2(pack_f32x2(__fmul_rn(v[i], alpha), __fmul_rn(v[i + 1], alpha)), pack_f32x2(b.x, b.y));
+            hi = add_f32x2(pack_f32x2(__fmul_rn(v[i + 2], alpha), __fmul_rn(v[i + 3], alpha)), pack_f32x2(b.z, b.w));
+        }
         if constexpr (ACT == 1 || ACT == 2) {
             gate_pair<ACT>(lo, v[i], v[i + 1]);
             gate_pair<ACT>(hi, v[i + 2], v[i + 3]);
@@ -200,30 +208,30 @@ __device__ __forceinline__ void finish_columns(float* v, const float* bias, floa
         }
     }
 }
-// 128 bytes of this lane's row into the warp's box of 32 rows (128-byte swizzle)
-__device__ __forceinline__ void stage_row(unsigned box, int lane, const uint32_t (&w)[32]) {
+// 64 bytes of this lane's row into the warp's box of 32 rows (64-byte swizzle: 16-byte pieces by bits 1-2 of the row)
+__device__ __forceinline__ void stage_row(unsigned box, int lane, const uint32_t (&w)[16]) {
 #pragma unroll
-    for (int c = 0; c < 8; ++c)
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + lane * 128 + ((c ^ (lane & 7)) << 4)), "r"(w[4 * c]), "r"(w[4 * c + 1]),
+    for (int c = 0; c < 4; ++c)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + lane * 64 + ((c ^ (lane >> 1 & 3)) << 4)), "r"(w[4 * c]), "r"(w[4 * c + 1]),
                      "r"(w[4 * c + 2]), "r"(w[4 * c + 3])
                      : "memory");
 }
 __device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int y, unsigned box) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(box)
                  : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
 // ------------------------------------------------------------------------------------- pair kernel --
-constexpr int kPairThreads = 320;
+constexpr int kPairThreads = 576;
 constexpr int kPairTile = 256;
-constexpr int kPairStages = 4;
+constexpr int kPairStages = 5;
 constexpr int kPairBufferBytes = 2 * kCodeBytes + 3 * kScaleBytes;   // a codes, b codes, a scales, b scales of all 256 columns
 constexpr int kPairColumns = 512;          // tensor memory: 256 accumulator columns, then 48 scale columns a buffer
 constexpr int kPairScaleColumns = 48;
-constexpr int kBoxBytes = 32 * 128;        // 32 rows of 128 bytes of the result
-constexpr int kPairWriters = 8;
-// + alignment of the swizzled tiles; two boxes and 128 bias values a writing warp
-constexpr int kPairSharedBytes = kPairStages * kPairBufferBytes + kPairWriters * (2 * kBoxBytes + 512) + 1024;
+constexpr int kWriters = 16;               // warps that write results: 32 rows x 64 columns of a tile each
+constexpr int kWriterColumns = 64;
+constexpr int kBoxBytes = 32 * 64;         // a stored box: 32 rows of 64 bytes
 static_assert(kPairTile + kPairStages * kPairScaleColumns <= kPairColumns, "scales do not fit tensor memory");
 
 struct PairControl {
@@ -231,15 +239,26 @@ struct PairControl {
     uint32_t tensor_base;
     volatile int abort;
 };
+struct __align__(1024) PairShared {        // fills an SM's shared memory, so it may not need room for alignment
+    uint8_t buffers[kPairStages][kPairBufferBytes];
+    uint8_t boxes[kWriters][kBoxBytes];
+    float bias[kWriters][kWriterColumns];
+    PairControl control;
+};
 
 template <int FORMAT, int ACT, int OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map,
                        const __grid_constant__ CUtensorMap a_scale_map, const __grid_constant__ CUtensorMap b_scale_map,
                        const __grid_constant__ CUtensorMap out_map, const LinearArgs p) {
-    extern __shared__ uint8_t dynamic_shared[];
-    __shared__ PairControl control;
-    const unsigned buffers = (shared_address(dynamic_shared) + 1023u) & ~1023u;
+    extern __shared__ __align__(1024) uint8_t dynamic_shared[];
+    PairShared& shared = *reinterpret_cast<PairShared*>(dynamic_shared);
+    PairControl& control = shared.control;
+    const unsigned buffers = shared_address(dynamic_shared);
+    if ((buffers & 1023u) != 0) {   // the same for every thread of the launch: no static shared memory precedes it
+        g_fp4_wait_gave_up = 1;
+        return;
+    }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned rank = cluster_rank();
     constexpr int kPerTile = FORMAT == VRB_NVFP4 ? 64 : 128;        // elements of k of a scale tile
@@ -248,7 +267,7 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
     if (threadIdx.x == 0) {
         for (int s = 0; s < kPairStages; ++s) { mbarrier_init(&control.full[s], 1); mbarrier_init(&control.empty[s], 1); }
         mbarrier_init(&control.done, 1);
-        mbarrier_init(&control.drained, 16);
+        mbarrier_init(&control.drained, 2 * kWriters);
         control.abort = 0;
         mbarrier_init_fence();
     }
@@ -334,72 +353,65 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
         }
     } else {
         const int quarter = warp & 3;                  // the 32 tensor-memory lanes this warp may read
-        const int side = (warp - 2) >> 2;              // its half of the columns
+        const int writer = warp - 2, group = writer >> 2;   // its 64 of the columns
         const float alpha = __fmul_rn(p.a_scale ? *p.a_scale : 1.0f, p.b_scale ? *p.b_scale : 1.0f);
-        const unsigned boxes = buffers + kPairStages * kPairBufferBytes + (warp - 2) * 2 * kBoxBytes;
-        uint8_t* generic = dynamic_shared + (buffers - shared_address(dynamic_shared)) + kPairStages * kPairBufferBytes;
-        float* scratch = reinterpret_cast<float*>(generic + (warp - 2) * 2 * kBoxBytes);
-        float* bias = reinterpret_cast<float*>(generic + kPairWriters * 2 * kBoxBytes) + (warp - 2) * 128;
-        int turn = 0;
+        const unsigned box = shared_address(shared.boxes[writer]);
+        float* scratch = reinterpret_cast<float*>(shared.boxes[writer]);
+        float* bias = shared.bias[writer];
         const unsigned drained = map_to_rank(shared_address(&control.drained), 0);
         unsigned phase = 0;
         for (int64_t t = pair; t < tiles; t += pairs) {
             int64_t row_tile, column_tile;
             tile_of(t, row_tiles, column_tiles, row_tile, column_tile);
-            const int64_t column0 = column_tile * kPairTile + side * 128;
+            const int64_t column0 = column_tile * kPairTile + group * kWriterColumns;
             if (p.bias) {   // before the wait: the loads are over when the accumulator is
+                __syncwarp();
 #pragma unroll
-                for (int c = 0; c < 128; c += 32) bias[c + lane] = column0 + c + lane < p.n ? load1(p.bias, p.bias_dt, column0 + c + lane) : 0.0f;
+                for (int c = 0; c < kWriterColumns; c += 32) bias[c + lane] = column0 + c + lane < p.n ? load1(p.bias, p.bias_dt, column0 + c + lane) : 0.0f;
             }
             if (!__all_sync(0xffffffffu, wait_barrier(&control.done, phase, &control.abort))) break;
             phase ^= 1u;
             fence_after();
-            float v[128];
-            const uint32_t address = base + side * 128 + (static_cast<uint32_t>(quarter * 32) << 16);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) read_columns(address + c * 32, v + c * 32);
+            float v[kWriterColumns];
+            const uint32_t address = base + group * kWriterColumns + (static_cast<uint32_t>(quarter * 32) << 16);
+            read_columns(address, v);
+            read_columns(address + 32, v + 32);
             wait_reads();
             fence_before();
             __syncwarp();
             if (lane == 0) arrive_cluster(drained);
             const int64_t row0 = row_tile * kPairTile + rank * kRows + quarter * 32;
-            const float* tile_bias = p.bias ? bias : nullptr;
             if (p.boxed) {
-                constexpr int N = OUT == VRB_BF16 ? 64 : 32;   // columns of a box
+                constexpr int N = OUT == VRB_BF16 ? 32 : 16;   // columns of a box
 #pragma unroll
-                for (int c = 0; c < 128; c += N) {
-                    finish_columns<ACT, N>(v + c, p.bias ? tile_bias + c : nullptr, alpha, p.activation);
-                    uint32_t w[32];
+                for (int c = 0; c < kWriterColumns; c += N) {
+                    finish_columns<ACT, N>(v + c, p.bias ? bias + c : nullptr, alpha, p.activation);
+                    uint32_t w[16];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) w[i] = OUT == VRB_BF16 ? pack_bf16x2(v[c + 2 * i % N], v[c + (2 * i + 1) % N]) : __float_as_uint(v[c + i]);
-                    const unsigned box = boxes + turn * kBoxBytes;
-                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");   // the box's store before last has read it
+                    for (int i = 0; i < 16; ++i) w[i] = OUT == VRB_BF16 ? pack_bf16x2(v[c + 2 * i % N], v[c + (2 * i + 1) % N]) : __float_as_uint(v[c + i % N]);
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the last store has read the box
                     __syncwarp();
                     stage_row(box, lane, w);
                     async_proxy_fence();
                     __syncwarp();
-                    if (lane == 0) {
-                        if (row0 < p.m && column0 + c < p.n) store_box(&out_map, static_cast<int>(column0 + c), static_cast<int>(row0), box);
-                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");   // an empty group too: the waits count them
-                    }
-                    turn ^= 1;
+                    if (lane == 0 && row0 < p.m && column0 + c < p.n) store_box(&out_map, static_cast<int>(column0 + c), static_cast<int>(row0), box);
                 }
             } else {
-                // rows off the 16-byte boundaries that a box needs: through scratch, so that a store covers 32 columns of a row
+                // rows off the 16-byte boundaries that a box needs: through scratch, 16 columns at a time, a lane to a column and
+                // every other row
                 const int height = static_cast<int>(p.m - row0 < 32 ? p.m - row0 : 32);
 #pragma unroll
-                for (int c = 0; c < 128; c += 32) {
-                    finish_columns<ACT, 32>(v + c, p.bias ? tile_bias + c : nullptr, alpha, p.activation);
+                for (int c = 0; c < kWriterColumns; c += 16) {
+                    finish_columns<ACT, 16>(v + c, p.bias ? bias + c : nullptr, alpha, p.activation);
                     __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) scratch[lane * 32 + (i ^ lane)] = v[c + i];
+                    for (int i = 0; i < 16; ++i) scratch[lane * 16 + (i ^ (lane >> 1 & 15))] = v[c + i];
                     __syncwarp();
-                    const int64_t column = column0 + c + lane;
+                    const int64_t column = column0 + c + (lane & 15);
                     if (column < p.n)
-                        for (int r = 0; r < height; ++r) store1(p.out, OUT, (row0 + r) * p.n + column, scratch[r * 32 + (lane ^ r)]);
+                        for (int r = lane >> 4; r < height; r += 2) store1(p.out, OUT, (row0 + r) * p.n + column, scratch[r * 16 + ((lane & 15) ^ (r >> 1 & 15))]);
                 }
             }
-            __syncwarp();
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
@@ -447,12 +459,12 @@ struct LinearMaps {
 
 template <int FORMAT, int ACT, int OUT>
 int launch_pair(const LinearMaps& maps, const LinearArgs& p, cudaStream_t s) {
-    static_assert(kPairSharedBytes + sizeof(PairControl) <= 227 * 1024, "ring does not fit shared memory");
-    const cudaError_t e = cudaFuncSetAttribute(fp4_linear_pair_kernel<FORMAT, ACT, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSharedBytes);
+    static_assert(sizeof(PairShared) <= 227 * 1024, "ring does not fit shared memory");
+    const cudaError_t e = cudaFuncSetAttribute(fp4_linear_pair_kernel<FORMAT, ACT, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(PairShared));
     VRB_REQUIRE(e == cudaSuccess, VRB_ERR_CUDA, "CUDA error: %s (fp4_linear)", cudaGetErrorString(e));
     const int64_t tiles = ((p.m + kPairTile - 1) / kPairTile) * ((p.n + kPairTile - 1) / kPairTile), pairs = sm_count() / 2;
     launch_overlapped(fp4_linear_pair_kernel<FORMAT, ACT, OUT>, dim3(static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs))), dim3(kPairThreads),
-                      kPairSharedBytes, s, maps.a, maps.b, maps.a_scales, maps.b_scales, maps.out, p);
+                      sizeof(PairShared), s, maps.a, maps.b, maps.a_scales, maps.b_scales, maps.out, p);
     return after_launch("fp4_linear");
 }
 template <int FORMAT, int OUT>
@@ -493,7 +505,7 @@ extern "C" int vrb_fp4_linear(int format, const void* a_codes, const void* a_sca
     VRB_REQUIRE(encode_codes(&maps.a, a_codes, rows_a, k, kRows) && encode_codes(&maps.b, b_codes, rows_b, k, kRows) &&
                     encode_scales(&maps.a_scales, format, a_scales, rows_a, k, 1) && encode_scales(&maps.b_scales, format, b_scales, rows_b, k, 2) &&
                     (!p.boxed || encode_2d(&maps.out, out_dtype == VRB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, out, rows_b,
-                                           rows_a, rows_b * element, static_cast<int>(128 / element), 32, CU_TENSOR_MAP_SWIZZLE_128B)),
+                                           rows_a, rows_b * element, static_cast<int>(64 / element), 32, CU_TENSOR_MAP_SWIZZLE_64B)),
                 VRB_ERR_UNSUPPORTED, "fp4_linear: the driver offers no tensor maps for these operands");
     cudaStream_t s = as_stream(stream);
     if (format == VRB_NVFP4) return out_dtype == VRB_BF16 ? launch_linear<VRB_NVFP4, VRB_BF16>(maps, p, s) : launch_linear<VRB_NVFP4, VRB_F32>(maps, p, s);
