@@ -14,6 +14,12 @@
 //   warps 2-17  take the accumulator out of tensor memory in one go (64 registers a thread: 256 accumulator columns and
 //               the scales leave no room for a second one), release it, and apply scale, bias and activation and
 //               store boxes of 32 rows through shared memory while the next tile's products run
+//
+// Split kernel, for few rows of a (single tokens) and for results of few tiles: CTAs on 128 rows of b x 16 to 128 rows of a, b's
+// rows on the accumulator's lanes so that even one row of a fills the tensor core's 128, and a cluster of up to eight CTAs
+// along k, which reads the weight with as many SMs as there are.  The CTAs of a cluster put their accumulators into shared
+// memory, and each adds a share of the columns over the cluster in rank order, so results do not depend on timing.
+//
 // Every wait is bounded: one that runs out sets a flag that the host can read and ends the CTA.
 #include <cuda.h>
 
@@ -100,6 +106,12 @@ __device__ __forceinline__ void load_box(unsigned dst, const CUtensorMap* map, i
                  : "memory");
 }
 
+__device__ __forceinline__ void load_own_box(unsigned dst, const CUtensorMap* map, int x, int y, unsigned barrier_address) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(barrier_address)
+                 : "memory");
+}
+
 // Shared-memory operand descriptors (start address, offsets in units of 16 bytes; bit 46: descriptor version).
 // Codes: rows of 128 bytes under the 128-byte swizzle, 8 rows = 1024 bytes apart.  Scale tile: 32 rows of 16 bytes, 8 rows
 // = 128 bytes apart, no swizzle.
@@ -127,6 +139,9 @@ __device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uin
     else VRB_MMA("1", "mxf4.block_scale.scale_vec::2X");
 #undef VRB_MMA
 }
+__device__ __forceinline__ void commit_one(uint64_t* barrier) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_address(barrier)) : "memory");
+}
 __device__ __forceinline__ void commit_pair(uint64_t* barrier) {   // arrives on the barrier at this offset in both CTAs
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(shared_address(barrier)),
                  "h"(static_cast<uint16_t>(3))
@@ -145,6 +160,14 @@ __device__ __forceinline__ void read_columns(uint32_t address, float* v) {
           "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
           "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
           "=r"(r[31])
+        : "r"(address));
+}
+__device__ __forceinline__ void read_columns16(uint32_t address, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(address));
 }
 __device__ __forceinline__ void wait_reads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -427,6 +450,192 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(kPairColumns));
 }
 
+// ------------------------------------------------------------------------------------ split kernel --
+constexpr int kSplitThreads = 192;
+constexpr int kSplitRing = 6;
+constexpr int kSplitColumns = 512;         // tensor memory: 128 accumulator columns, then 32 scale columns a buffer
+constexpr int kMostSplits = 8;             // portable cluster size
+
+struct SplitArgs {
+    LinearArgs linear;
+    int columns;               // rows of a of a tile: 16, 32, 64 or 128
+    int ring;                  // buffers
+    int splits;                // CTAs along k: the cluster
+    int stages;                // of all of k
+};
+struct SplitControl {
+    uint64_t full[kSplitRing], empty[kSplitRing], done;
+    uint32_t tensor_base;
+    volatile int abort;
+};
+
+__device__ __forceinline__ float load_cluster(unsigned address) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(address) : "memory");
+    return v;
+}
+// act(alpha acc + bias) as in finish_columns, one value
+__device__ __forceinline__ float finish_value(const LinearArgs& p, float accumulation, float alpha, float bias) {
+    const float y = p.activation == VRB_SILU || p.activation == VRB_GELU_TANH ? __fmaf_rn(accumulation, alpha, bias)
+                                                                            : __fadd_rn(__fmul_rn(accumulation, alpha), bias);
+    if (p.activation == VRB_NO_ACTIVATION) return y;
+    float out, unused;
+    if (p.activation == VRB_SILU) gate_pair<1>(pack_f32x2(y, 0.0f), out, unused);
+    else if (p.activation == VRB_GELU_TANH) gate_pair<2>(pack_f32x2(y, 0.0f), out, unused);
+    else out = activation_value(p.activation, y);
+    return out;
+}
+
+template <int FORMAT>
+__global__ void __launch_bounds__(kSplitThreads, 1)
+fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map,
+                        const __grid_constant__ CUtensorMap a_scale_map, const __grid_constant__ CUtensorMap b_scale_map, const SplitArgs q) {
+    extern __shared__ uint8_t dynamic_shared[];
+    __shared__ SplitControl control;
+    const LinearArgs& p = q.linear;
+    const unsigned buffers = (shared_address(dynamic_shared) + 1023u) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int kPerTile = FORMAT == VRB_NVFP4 ? 64 : 128;
+    constexpr int kTiles = kStageElements / kPerTile;
+    const unsigned a_bytes = q.columns * kStageBytes, buffer_bytes = kCodeBytes + 2 * kScaleBytes + ((a_bytes + 1023u) & ~1023u);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kSplitRing; ++s) { mbarrier_init(&control.full[s], 1); mbarrier_init(&control.empty[s], 1); }
+        mbarrier_init(&control.done, 1);
+        control.abort = 0;
+        mbarrier_init_fence();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(&control.tensor_base)), "r"(kSplitColumns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t base = control.tensor_base;
+    pdl_wait();
+
+    // blockIdx.x = (column tile of b * tiles of a + tile of a) * splits + rank
+    const int rank = static_cast<int>(blockIdx.x % q.splits);
+    const int64_t tile = blockIdx.x / q.splits, a_tiles = (p.m + q.columns - 1) / q.columns;
+    const int64_t b0 = tile / a_tiles * kRows, a0 = tile % a_tiles * q.columns;
+    const int first = static_cast<int>(static_cast<int64_t>(q.stages) * rank / q.splits), last = static_cast<int>(static_cast<int64_t>(q.stages) * (rank + 1) / q.splits);
+
+    if (warp == 0) {
+        int slot = 0;
+        unsigned phase = 1;
+        for (int stage = first; stage < last; ++stage) {
+            if (!wait_barrier(&control.empty[slot], phase, &control.abort)) break;
+            if (elect_one()) {
+                const unsigned buffer = buffers + slot * buffer_bytes, full = shared_address(&control.full[slot]);
+                mbarrier_expect_bytes(&control.full[slot], kCodeBytes + a_bytes + 2 * kTiles * 512);
+                load_own_box(buffer, &b_map, stage * kStageBytes, static_cast<int>(b0), full);
+                load_own_box(buffer + kCodeBytes, &b_scale_map, stage * kTiles * 64, static_cast<int>(b0 / 128), full);
+                load_own_box(buffer + kCodeBytes + kScaleBytes, &a_scale_map, stage * kTiles * 64, static_cast<int>(a0 / 128), full);
+                load_own_box(buffer + kCodeBytes + 2 * kScaleBytes, &a_map, stage * kStageBytes, static_cast<int>(a0), full);
+            }
+            __syncwarp();
+            if (++slot == q.ring) { slot = 0; phase ^= 1u; }
+        }
+    } else if (warp == 1) {
+        const uint32_t instruction = instruction_descriptor<FORMAT>(kRows, q.columns);
+        const uint32_t a_column = static_cast<uint32_t>(a0 % 128) / 32;   // where the tile's scales begin within the 128-row scale tile
+        int slot = 0;
+        unsigned phase = 0;
+        for (int stage = first; stage < last; ++stage) {
+            if (!wait_barrier(&control.full[slot], phase, &control.abort)) break;
+            fence_after();
+            if (elect_one()) {
+                const unsigned buffer = buffers + slot * buffer_bytes;
+                const uint32_t sb = base + 128 + slot * 32, sa = sb + 16;
+                const uint64_t b_codes = kCodeDescriptor | ((buffer & 0x3ffffu) >> 4), a_codes = b_codes + ((kCodeBytes + 2 * kScaleBytes) >> 4);
+                const uint64_t scales = kScaleDescriptor | (((buffer + kCodeBytes) & 0x3ffffu) >> 4);
+                const int64_t left = p.k - static_cast<int64_t>(stage) * kStageElements;
+                const int steps = left < kStageElements ? static_cast<int>((left + 63) / 64) : 4;
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) {
+                    copy_scales<1>(sb + i * 4, scales + i * 32);
+                    copy_scales<1>(sa + i * 4, scales + (kScaleBytes >> 4) + i * 32);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i < steps) {
+                        constexpr int per = kPerTile / 64;
+                        const uint32_t half = FORMAT == VRB_MXFP4 ? static_cast<uint32_t>(i & 1) * 2u : 0u;
+                        multiply<FORMAT, 1>(base, b_codes + i * 2, a_codes + i * 2, instruction | (half << 4) | (half << 29), sb + i / per * 4,
+                                            sa + i / per * 4 + a_column, stage > first || i > 0 ? 1u : 0u);
+                    }
+                commit_one(&control.empty[slot]);
+                if (stage == last - 1) commit_one(&control.done);
+            }
+            __syncwarp();
+            if (++slot == q.ring) { slot = 0; phase ^= 1u; }
+        }
+    }
+    const bool writer = warp >= 2;
+    const int row = (warp & 3) * 32 + lane;            // of b within the tile: the tensor-memory lane
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const float alpha = __fmul_rn(p.a_scale ? *p.a_scale : 1.0f, p.b_scale ? *p.b_scale : 1.0f);
+    const float bias = p.bias && writer && b0 + row < p.n ? load1(p.bias, p.bias_dt, b0 + row) : 0.0f;
+    const int64_t height = p.m - a0 < q.columns ? p.m - a0 : q.columns;
+    bool ok = true;
+    if (writer) {
+        ok = __all_sync(0xffffffffu, wait_barrier(&control.done, 0, &control.abort));
+        if (ok) fence_after();
+        if (ok && q.splits == 1) {
+            for (int c = 0; c < height; c += 16) {
+                float v[16];
+                read_columns16(base + lanes + c, v);
+                wait_reads();
+                if (b0 + row < p.n)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (c + i < height) store1(p.out, p.out_dt, (a0 + c + i) * p.n + b0 + row, finish_value(p, v[i], alpha, bias));
+                __syncwarp();
+            }
+        } else if (ok) {
+            // all copies into the ring and all products out of it are over: its memory takes the accumulator, 128 floats a column
+            for (int c = 0; c < q.columns; c += 16) {
+                float v[16];
+                read_columns16(base + lanes + c, v);
+                wait_reads();
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(buffers + ((c + i) * 128 + row) * 4), "f"(v[i]) : "memory");
+            }
+        }
+    }
+    if (q.splits > 1) {
+        __syncwarp();
+        cluster_sync();
+        if (writer && ok && b0 + row < p.n) {
+            const int share = (static_cast<int>(height) + q.splits - 1) / q.splits, end = min(static_cast<int>(height), (rank + 1) * share);
+            for (int c = rank * share; c < end; c += 4) {
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (int r = 0; r < q.splits; ++r) {
+                    const unsigned remote = map_to_rank(buffers, r) + (c * 128 + row) * 4;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (c + i < end) sum[i] += load_cluster(remote + i * 512);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (c + i < end) store1(p.out, p.out_dt, (a0 + c + i) * p.n + b0 + row, finish_value(p, sum[i], alpha, bias));
+            }
+        }
+        __syncwarp();
+        cluster_sync();        // no CTA's memory goes while another reads it
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    if (control.abort) {       // let copies and products in flight end before their memory goes
+        const unsigned long long start = now_ns();
+        for (int i = 0; i < 100000 && now_ns() - start < 20000000ull; ++i) __nanosleep(1000);
+    }
+    fence_after();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(kSplitColumns));
+}
+
 // ----------------------------------------------------------------------------------------- host side --
 using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -467,6 +676,68 @@ int launch_pair(const LinearMaps& maps, const LinearArgs& p, cudaStream_t s) {
                       sizeof(PairShared), s, maps.a, maps.b, maps.a_scales, maps.b_scales, maps.out, p);
     return after_launch("fp4_linear");
 }
+// Which kernel, and the split kernel's tile and cluster: the least of the times that a model gives, in cycles.  Measured on B200:
+// a stage of the pair kernel takes 560 (products 512), of the split kernel the time its bytes need at 72 a cycle and
+// SM; a tile costs about 1500 beyond its stages (start, drain), a split tile 2000, and another 1200 to meet in the cluster.
+struct LinearPlan {
+    int columns;   // 0: pair kernel
+    int splits;
+};
+LinearPlan plan_linear(int64_t m, int64_t n, int stages) {
+    const int64_t sms = sm_count();
+    auto ceil_div = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    LinearPlan best{0, 1};
+    const int64_t pair_tiles = ceil_div(m, kPairTile) * ceil_div(n, kPairTile);
+    int64_t least = ceil_div(pair_tiles, sms / 2 > 0 ? sms / 2 : 1) * (static_cast<int64_t>(stages) * 560 + 1500);
+    for (int columns = 16; columns <= 128; columns *= 2) {
+        if (columns <= 32 && m > columns) continue;   // narrower tiles than 64 would begin inside a scale word's lanes
+        const int64_t tiles = ceil_div(m, columns) * ceil_div(n, kRows), stage = (kCodeBytes + 2 * kScaleBytes + columns * kStageBytes) / 72;
+        for (int splits = 1; splits <= kMostSplits && splits <= stages; ++splits) {
+            // clusters above 4 leave SMs of some processor groups idle
+            const int64_t room = splits > 4 ? sms * 7 / 8 : sms, ctas = tiles * splits;
+            const int64_t time = ceil_div(ctas, room) * (ceil_div(stages, splits) * stage + 2000 + (splits > 1 ? 1200 : 0));
+            if (time < least) { least = time; best = {columns, splits}; }
+        }
+        if (m <= columns) break;
+    }
+    return best;
+}
+
+template <int FORMAT>
+int launch_split(const LinearMaps& maps, const LinearArgs& p, const LinearPlan& plan, cudaStream_t s) {
+    SplitArgs q{};
+    q.linear = p;
+    q.columns = plan.columns;
+    q.splits = plan.splits;
+    q.stages = static_cast<int>((p.k + kStageElements - 1) / kStageElements);
+    const int own = (q.stages + q.splits - 1) / q.splits;
+    q.ring = own < kSplitRing ? own : kSplitRing;
+    const size_t buffer = kCodeBytes + 2 * kScaleBytes + ((static_cast<size_t>(q.columns) * kStageBytes + 1023) & ~size_t{1023});
+    size_t bytes = q.ring * buffer;
+    if (q.splits > 1 && bytes < static_cast<size_t>(q.columns) * 512) bytes = static_cast<size_t>(q.columns) * 512;
+    bytes += 1024;
+    static_assert(kSplitRing * (2 * kCodeBytes + 2 * kScaleBytes) + 1024 + sizeof(SplitControl) <= 227 * 1024, "ring does not fit shared memory");
+    cudaError_t e = cudaFuncSetAttribute(fp4_linear_split_kernel<FORMAT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         kSplitRing * (2 * kCodeBytes + 2 * kScaleBytes) + 1024);
+    VRB_REQUIRE(e == cudaSuccess, VRB_ERR_CUDA, "CUDA error: %s (fp4_linear)", cudaGetErrorString(e));
+    const int64_t tiles = ((p.m + q.columns - 1) / q.columns) * ((p.n + kRows - 1) / kRows);
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(static_cast<unsigned>(tiles * q.splits));
+    config.blockDim = dim3(kSplitThreads);
+    config.dynamicSmemBytes = bytes;
+    config.stream = s;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeClusterDimension;
+    attributes[0].val.clusterDim.x = static_cast<unsigned>(q.splits);
+    attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+    attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[1].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attributes;
+    config.numAttrs = g_launch_overlap.load(std::memory_order_relaxed) != 0 ? 2 : 1;
+    cudaLaunchKernelEx(&config, fp4_linear_split_kernel<FORMAT>, maps.a, maps.b, maps.a_scales, maps.b_scales, q);   // an error stays for after_launch()
+    return after_launch("fp4_linear");
+}
+
 template <int FORMAT, int OUT>
 int launch_linear(const LinearMaps& maps, const LinearArgs& p, cudaStream_t s) {
     if (p.activation == VRB_NO_ACTIVATION) return launch_pair<FORMAT, 0, OUT>(maps, p, s);
@@ -501,13 +772,16 @@ extern "C" int vrb_fp4_linear(int format, const void* a_codes, const void* a_sca
     p.m = rows_a; p.n = rows_b; p.k = k;
     const int64_t element = static_cast<int64_t>(dtype_bytes(out_dtype));
     p.boxed = aligned16(out) && rows_b * element % 16 == 0;
+    const LinearPlan plan = plan_linear(rows_a, rows_b, static_cast<int>((k + kStageElements - 1) / kStageElements));
+    const bool pair = plan.columns == 0;
     LinearMaps maps{};
-    VRB_REQUIRE(encode_codes(&maps.a, a_codes, rows_a, k, kRows) && encode_codes(&maps.b, b_codes, rows_b, k, kRows) &&
-                    encode_scales(&maps.a_scales, format, a_scales, rows_a, k, 1) && encode_scales(&maps.b_scales, format, b_scales, rows_b, k, 2) &&
-                    (!p.boxed || encode_2d(&maps.out, out_dtype == VRB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, out, rows_b,
-                                           rows_a, rows_b * element, static_cast<int>(64 / element), 32, CU_TENSOR_MAP_SWIZZLE_64B)),
+    VRB_REQUIRE(encode_codes(&maps.a, a_codes, rows_a, k, pair ? kRows : plan.columns) && encode_codes(&maps.b, b_codes, rows_b, k, kRows) &&
+                    encode_scales(&maps.a_scales, format, a_scales, rows_a, k, 1) && encode_scales(&maps.b_scales, format, b_scales, rows_b, k, pair ? 2 : 1) &&
+                    (!pair || !p.boxed || encode_2d(&maps.out, out_dtype == VRB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, out, rows_b,
+                                                    rows_a, rows_b * element, static_cast<int>(64 / element), 32, CU_TENSOR_MAP_SWIZZLE_64B)),
                 VRB_ERR_UNSUPPORTED, "fp4_linear: the driver offers no tensor maps for these operands");
     cudaStream_t s = as_stream(stream);
+    if (!pair) return format == VRB_NVFP4 ? launch_split<VRB_NVFP4>(maps, p, plan, s) : launch_split<VRB_MXFP4>(maps, p, plan, s);
     if (format == VRB_NVFP4) return out_dtype == VRB_BF16 ? launch_linear<VRB_NVFP4, VRB_BF16>(maps, p, s) : launch_linear<VRB_NVFP4, VRB_F32>(maps, p, s);
     return out_dtype == VRB_BF16 ? launch_linear<VRB_MXFP4, VRB_BF16>(maps, p, s) : launch_linear<VRB_MXFP4, VRB_F32>(maps, p, s);
 }
