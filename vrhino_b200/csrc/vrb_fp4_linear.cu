@@ -48,6 +48,7 @@ struct LinearArgs {
     int64_t k;
     int bias_dt, out_dt, activation;
     int boxed;                 // rows of out lie on 16-byte boundaries: stored as boxes
+    int quads;                 // and on boundaries of four elements
 };
 
 __device__ __forceinline__ unsigned long long now_ns() {
@@ -469,24 +470,12 @@ struct SplitControl {
     volatile int abort;
 };
 
-__device__ __forceinline__ float load_cluster(unsigned address) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(address) : "memory");
+__device__ __forceinline__ float4 load_cluster(unsigned address) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(address) : "memory");
     return v;
 }
-// act(alpha acc + bias) as in finish_columns, one value
-__device__ __forceinline__ float finish_value(const LinearArgs& p, float accumulation, float alpha, float bias) {
-    const float y = p.activation == VRB_SILU || p.activation == VRB_GELU_TANH ? __fmaf_rn(accumulation, alpha, bias)
-                                                                            : __fadd_rn(__fmul_rn(accumulation, alpha), bias);
-    if (p.activation == VRB_NO_ACTIVATION) return y;
-    float out, unused;
-    if (p.activation == VRB_SILU) gate_pair<1>(pack_f32x2(y, 0.0f), out, unused);
-    else if (p.activation == VRB_GELU_TANH) gate_pair<2>(pack_f32x2(y, 0.0f), out, unused);
-    else out = activation_value(p.activation, y);
-    return out;
-}
-
-template <int FORMAT>
+template <int FORMAT, int ACT>
 __global__ void __launch_bounds__(kSplitThreads, 1)
 fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map,
                         const __grid_constant__ CUtensorMap a_scale_map, const __grid_constant__ CUtensorMap b_scale_map, const SplitArgs q) {
@@ -571,60 +560,56 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
             if (++slot == q.ring) { slot = 0; phase ^= 1u; }
         }
     }
-    const bool writer = warp >= 2;
-    const int row = (warp & 3) * 32 + lane;            // of b within the tile: the tensor-memory lane
-    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const float alpha = __fmul_rn(p.a_scale ? *p.a_scale : 1.0f, p.b_scale ? *p.b_scale : 1.0f);
-    const float bias = p.bias && writer && b0 + row < p.n ? load1(p.bias, p.bias_dt, b0 + row) : 0.0f;
-    const int64_t height = p.m - a0 < q.columns ? p.m - a0 : q.columns;
-    bool ok = true;
-    if (writer) {
-        ok = __all_sync(0xffffffffu, wait_barrier(&control.done, 0, &control.abort));
-        if (ok) fence_after();
-        if (ok && q.splits == 1) {
-            for (int c = 0; c < height; c += 16) {
-                float v[16];
-                read_columns16(base + lanes + c, v);
-                wait_reads();
-                if (b0 + row < p.n)
+    const int height = static_cast<int>(p.m - a0 < q.columns ? p.m - a0 : q.columns);
+    if (warp >= 2 && __all_sync(0xffffffffu, wait_barrier(&control.done, 0, &control.abort))) {
+        // all copies into the ring and all products out of it are over: its memory takes the accumulator, 128 floats a column
+        fence_after();
+        const unsigned mine = buffers + ((warp & 3) * 32 + lane) * 4;       // the tensor-memory lane is the row of b
+        for (int c = 0; c < height; c += 16) {
+            float v[16];
+            read_columns16(base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + c, v);
+            wait_reads();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (c + i < height) store1(p.out, p.out_dt, (a0 + c + i) * p.n + b0 + row, finish_value(p, v[i], alpha, bias));
-                __syncwarp();
-            }
-        } else if (ok) {
-            // all copies into the ring and all products out of it are over: its memory takes the accumulator, 128 floats a column
-            for (int c = 0; c < q.columns; c += 16) {
-                float v[16];
-                read_columns16(base + lanes + c, v);
-                wait_reads();
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(buffers + ((c + i) * 128 + row) * 4), "f"(v[i]) : "memory");
-            }
+            for (int i = 0; i < 16; ++i) asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + (c + i) * 512), "f"(v[i]) : "memory");
         }
     }
-    if (q.splits > 1) {
-        __syncwarp();
-        cluster_sync();
-        if (writer && ok && b0 + row < p.n) {
-            const int share = (static_cast<int>(height) + q.splits - 1) / q.splits, end = min(static_cast<int>(height), (rank + 1) * share);
-            for (int c = rank * share; c < end; c += 4) {
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                for (int r = 0; r < q.splits; ++r) {
-                    const unsigned remote = map_to_rank(buffers, r) + (c * 128 + row) * 4;
+    __syncwarp();
+    if (q.splits > 1) cluster_sync(); else __syncthreads();
+    {
+        // this CTA's share of the columns, four rows of b to a thread: a warp writes 128 consecutive elements of a row of the result
+        const float alpha = __fmul_rn(p.a_scale ? *p.a_scale : 1.0f, p.b_scale ? *p.b_scale : 1.0f);
+        const int share = (height + q.splits - 1) / q.splits, begin = rank * share, end = min(height, begin + share);
+        const int64_t n0 = b0 + lane * 4;
+        if (n0 < p.n && !control.abort) {
+            __align__(16) float bias[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (c + i < end) sum[i] += load_cluster(remote + i * 512);
+            for (int e = 0; e < 4; ++e) bias[e] = p.bias && n0 + e < p.n ? load1(p.bias, p.bias_dt, n0 + e) : 0.0f;
+#pragma unroll 1
+            for (int c = begin + warp; c < end; c += kSplitThreads / 32) {
+                float4 part[kMostSplits];
+#pragma unroll
+                for (int r = 0; r < kMostSplits; ++r)
+                    if (r < q.splits) part[r] = load_cluster((q.splits > 1 ? map_to_rank(buffers, r) : buffers) + (c * 128 + lane * 4) * 4);
+                float y[4] = {part[0].x, part[0].y, part[0].z, part[0].w};
+#pragma unroll
+                for (int r = 1; r < kMostSplits; ++r)
+                    if (r < q.splits) { y[0] += part[r].x; y[1] += part[r].y; y[2] += part[r].z; y[3] += part[r].w; }
+                finish_columns<ACT, 4>(y, bias, alpha, p.activation);
+                const int64_t at = (a0 + c) * p.n + n0;
+                if (p.quads && p.out_dt == VRB_BF16) {
+                    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+                } else if (p.quads) {
+                    *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(y[0], y[1], y[2], y[3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (n0 + e < p.n) store1(p.out, p.out_dt, at + e, y[e]);
                 }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (c + i < end) store1(p.out, p.out_dt, (a0 + c + i) * p.n + b0 + row, finish_value(p, sum[i], alpha, bias));
             }
         }
-        __syncwarp();
-        cluster_sync();        // no CTA's memory goes while another reads it
     }
+    __syncwarp();
+    if (q.splits > 1) cluster_sync();   // no CTA's memory goes while another reads it
     __syncwarp();
     fence_before();
     __syncthreads();
@@ -703,7 +688,7 @@ LinearPlan plan_linear(int64_t m, int64_t n, int stages) {
     return best;
 }
 
-template <int FORMAT>
+template <int FORMAT, int ACT>
 int launch_split(const LinearMaps& maps, const LinearArgs& p, const LinearPlan& plan, cudaStream_t s) {
     SplitArgs q{};
     q.linear = p;
@@ -714,10 +699,10 @@ int launch_split(const LinearMaps& maps, const LinearArgs& p, const LinearPlan& 
     q.ring = own < kSplitRing ? own : kSplitRing;
     const size_t buffer = kCodeBytes + 2 * kScaleBytes + ((static_cast<size_t>(q.columns) * kStageBytes + 1023) & ~size_t{1023});
     size_t bytes = q.ring * buffer;
-    if (q.splits > 1 && bytes < static_cast<size_t>(q.columns) * 512) bytes = static_cast<size_t>(q.columns) * 512;
+    if (bytes < static_cast<size_t>(q.columns) * 512) bytes = static_cast<size_t>(q.columns) * 512;
     bytes += 1024;
     static_assert(kSplitRing * (2 * kCodeBytes + 2 * kScaleBytes) + 1024 + sizeof(SplitControl) <= 227 * 1024, "ring does not fit shared memory");
-    cudaError_t e = cudaFuncSetAttribute(fp4_linear_split_kernel<FORMAT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(fp4_linear_split_kernel<FORMAT, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          kSplitRing * (2 * kCodeBytes + 2 * kScaleBytes) + 1024);
     VRB_REQUIRE(e == cudaSuccess, VRB_ERR_CUDA, "CUDA error: %s (fp4_linear)", cudaGetErrorString(e));
     const int64_t tiles = ((p.m + q.columns - 1) / q.columns) * ((p.n + kRows - 1) / kRows);
@@ -734,8 +719,16 @@ int launch_split(const LinearMaps& maps, const LinearArgs& p, const LinearPlan& 
     attributes[1].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = attributes;
     config.numAttrs = g_launch_overlap.load(std::memory_order_relaxed) != 0 ? 2 : 1;
-    cudaLaunchKernelEx(&config, fp4_linear_split_kernel<FORMAT>, maps.a, maps.b, maps.a_scales, maps.b_scales, q);   // an error stays for after_launch()
+    cudaLaunchKernelEx(&config, fp4_linear_split_kernel<FORMAT, ACT>, maps.a, maps.b, maps.a_scales, maps.b_scales, q);   // an error stays for after_launch()
     return after_launch("fp4_linear");
+}
+
+template <int FORMAT>
+int launch_split(const LinearMaps& maps, const LinearArgs& p, const LinearPlan& plan, cudaStream_t s) {
+    if (p.activation == VRB_NO_ACTIVATION) return launch_split<FORMAT, 0>(maps, p, plan, s);
+    if (p.activation == VRB_SILU) return launch_split<FORMAT, 1>(maps, p, plan, s);
+    if (p.activation == VRB_GELU_TANH) return launch_split<FORMAT, 2>(maps, p, plan, s);
+    return launch_split<FORMAT, 3>(maps, p, plan, s);
 }
 
 template <int FORMAT, int OUT>
@@ -772,6 +765,7 @@ extern "C" int vrb_fp4_linear(int format, const void* a_codes, const void* a_sca
     p.m = rows_a; p.n = rows_b; p.k = k;
     const int64_t element = static_cast<int64_t>(dtype_bytes(out_dtype));
     p.boxed = aligned16(out) && rows_b * element % 16 == 0;
+    p.quads = reinterpret_cast<uintptr_t>(out) % (4 * element) == 0 && rows_b % 4 == 0;
     const LinearPlan plan = plan_linear(rows_a, rows_b, static_cast<int>((k + kStageElements - 1) / kStageElements));
     const bool pair = plan.columns == 0;
     LinearMaps maps{};
