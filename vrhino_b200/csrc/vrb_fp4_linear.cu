@@ -283,7 +283,7 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
         g_fp4_wait_gave_up = 1;
         return;
     }
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // known to be the same for a warp
     const unsigned rank = cluster_rank();
     constexpr int kPerTile = FORMAT == VRB_NVFP4 ? 64 : 128;        // elements of k of a scale tile
     constexpr int kTiles = kStageElements / kPerTile;               // scale tiles of 128 rows a stage
@@ -483,7 +483,7 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
     __shared__ SplitControl control;
     const LinearArgs& p = q.linear;
     const unsigned buffers = (shared_address(dynamic_shared) + 1023u) & ~1023u;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // known to be the same for a warp
     constexpr int kPerTile = FORMAT == VRB_NVFP4 ? 64 : 128;
     constexpr int kTiles = kStageElements / kPerTile;
     const unsigned a_bytes = q.columns * kStageBytes, buffer_bytes = kCodeBytes + 2 * kScaleBytes + ((a_bytes + 1023u) & ~1023u);
@@ -530,33 +530,31 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
         const uint32_t a_column = static_cast<uint32_t>(a0 % 128) / 32;   // where the tile's scales begin within the 128-row scale tile
         int slot = 0;
         unsigned phase = 0;
-        for (int stage = first; stage < last; ++stage) {
+        // one thread for the whole loop: electing one a stage takes as long as the products of a narrow tile
+        if (elect_one()) for (int stage = first; stage < last; ++stage) {
             if (!wait_barrier(&control.full[slot], phase, &control.abort)) break;
             fence_after();
-            if (elect_one()) {
-                const unsigned buffer = buffers + slot * buffer_bytes;
-                const uint32_t sb = base + 128 + slot * 32, sa = sb + 16;
-                const uint64_t b_codes = kCodeDescriptor | ((buffer & 0x3ffffu) >> 4), a_codes = b_codes + ((kCodeBytes + 2 * kScaleBytes) >> 4);
-                const uint64_t scales = kScaleDescriptor | (((buffer + kCodeBytes) & 0x3ffffu) >> 4);
-                const int64_t left = p.k - static_cast<int64_t>(stage) * kStageElements;
-                const int steps = left < kStageElements ? static_cast<int>((left + 63) / 64) : 4;
+            const unsigned buffer = buffers + slot * buffer_bytes;
+            const uint32_t sb = base + 128 + slot * 32, sa = sb + 16;
+            const uint64_t b_codes = kCodeDescriptor | ((buffer & 0x3ffffu) >> 4), a_codes = b_codes + ((kCodeBytes + 2 * kScaleBytes) >> 4);
+            const uint64_t scales = kScaleDescriptor | (((buffer + kCodeBytes) & 0x3ffffu) >> 4);
+            const int64_t left = p.k - static_cast<int64_t>(stage) * kStageElements;
+            const int steps = left < kStageElements ? static_cast<int>((left + 63) / 64) : 4;
 #pragma unroll
-                for (int i = 0; i < kTiles; ++i) {
-                    copy_scales<1>(sb + i * 4, scales + i * 32);
-                    copy_scales<1>(sa + i * 4, scales + (kScaleBytes >> 4) + i * 32);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (i < steps) {
-                        constexpr int per = kPerTile / 64;
-                        const uint32_t half = FORMAT == VRB_MXFP4 ? static_cast<uint32_t>(i & 1) * 2u : 0u;
-                        multiply<FORMAT, 1>(base, b_codes + i * 2, a_codes + i * 2, instruction | (half << 4) | (half << 29), sb + i / per * 4,
-                                            sa + i / per * 4 + a_column, stage > first || i > 0 ? 1u : 0u);
-                    }
-                commit_one(&control.empty[slot]);
-                if (stage == last - 1) commit_one(&control.done);
+            for (int i = 0; i < kTiles; ++i) {
+                copy_scales<1>(sb + i * 4, scales + i * 32);
+                copy_scales<1>(sa + i * 4, scales + (kScaleBytes >> 4) + i * 32);
             }
-            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < steps) {
+                    constexpr int per = kPerTile / 64;
+                    const uint32_t half = FORMAT == VRB_MXFP4 ? static_cast<uint32_t>(i & 1) * 2u : 0u;
+                    multiply<FORMAT, 1>(base, b_codes + i * 2, a_codes + i * 2, instruction | (half << 4) | (half << 29), sb + i / per * 4,
+                                        sa + i / per * 4 + a_column, stage > first || i > 0 ? 1u : 0u);
+                }
+            commit_one(&control.empty[slot]);
+            if (stage == last - 1) commit_one(&control.done);
             if (++slot == q.ring) { slot = 0; phase ^= 1u; }
         }
     }
