@@ -174,10 +174,9 @@ __device__ __forceinline__ void read_columns16(uint32_t address, float* v) {
 __device__ __forceinline__ void wait_reads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // The tile of a linear index: bands of kBand row tiles, row tiles innermost, so that the CTAs at work share operand rows
-__device__ __forceinline__ void tile_of(int64_t index, int64_t row_tiles, int64_t column_tiles, int64_t& row_tile, int64_t& column_tile) {
-    const int64_t band = index / (kBand * column_tiles), first = band * kBand;
-    const int64_t height = row_tiles - first < kBand ? row_tiles - first : kBand;
-    const int64_t within = index - band * kBand * column_tiles;
+__device__ __forceinline__ void tile_of(unsigned index, unsigned row_tiles, unsigned column_tiles, unsigned& row_tile, unsigned& column_tile) {
+    const unsigned band = index / (kBand * column_tiles), first = band * kBand;
+    const unsigned height = min(row_tiles - first, static_cast<unsigned>(kBand)), within = index - band * kBand * column_tiles;
     column_tile = within / height;
     row_tile = first + within - column_tile * height;
 }
@@ -306,16 +305,17 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
     const uint32_t base = control.tensor_base;
     pdl_wait();
 
-    const int64_t row_tiles = (p.m + kPairTile - 1) / kPairTile, column_tiles = (p.n + kPairTile - 1) / kPairTile, tiles = row_tiles * column_tiles;
+    const unsigned row_tiles = static_cast<unsigned>((p.m + kPairTile - 1) / kPairTile), column_tiles = static_cast<unsigned>((p.n + kPairTile - 1) / kPairTile);
+    const unsigned tiles = row_tiles * column_tiles;
     const int stages = static_cast<int>((p.k + kStageElements - 1) / kStageElements);
-    const int64_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const unsigned pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if (warp == 0) {
         int slot = 0;
         unsigned phase = 1;
         bool ok = true;
-        for (int64_t t = pair; ok && t < tiles; t += pairs) {
-            int64_t row_tile, column_tile;
+        for (unsigned t = pair; ok && t < tiles; t += pairs) {
+            unsigned row_tile, column_tile;
             tile_of(t, row_tiles, column_tiles, row_tile, column_tile);
             for (int stage = 0; stage < stages; ++stage) {
                 if (!wait_barrier(&control.empty[slot], phase, &control.abort)) { ok = false; break; }
@@ -338,7 +338,7 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
             int slot = 0;
             unsigned phase = 0, drained_phase = 1;
             bool ok = true;
-            for (int64_t t = pair; ok && t < tiles; t += pairs) {
+            for (unsigned t = pair; ok && t < tiles; t += pairs) {
                 if (!wait_barrier(&control.drained, drained_phase, &control.abort)) break;
                 drained_phase ^= 1u;
                 fence_after();
@@ -384,10 +384,10 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
         float* bias = shared.bias[writer];
         const unsigned drained = map_to_rank(shared_address(&control.drained), 0);
         unsigned phase = 0;
-        for (int64_t t = pair; t < tiles; t += pairs) {
-            int64_t row_tile, column_tile;
+        for (unsigned t = pair; t < tiles; t += pairs) {
+            unsigned row_tile, column_tile;
             tile_of(t, row_tiles, column_tiles, row_tile, column_tile);
-            const int64_t column0 = column_tile * kPairTile + group * kWriterColumns;
+            const int64_t column0 = static_cast<int64_t>(column_tile) * kPairTile + group * kWriterColumns;
             if (p.bias) {   // before the wait: the loads are over when the accumulator is
                 __syncwarp();
 #pragma unroll
@@ -404,7 +404,7 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
             fence_before();
             __syncwarp();
             if (lane == 0) arrive_cluster(drained);
-            const int64_t row0 = row_tile * kPairTile + rank * kRows + quarter * 32;
+            const int64_t row0 = static_cast<int64_t>(row_tile) * kPairTile + rank * kRows + quarter * 32;
             if (p.boxed) {
                 constexpr int N = OUT == VRB_BF16 ? 32 : 16;   // columns of a box
 #pragma unroll
@@ -463,6 +463,7 @@ struct SplitArgs {
     int ring;                  // buffers
     int splits;                // CTAs along k: the cluster
     int stages;                // of all of k
+    unsigned a_tiles;
 };
 struct SplitControl {
     uint64_t full[kSplitRing], empty[kSplitRing], done;
@@ -472,7 +473,7 @@ struct SplitControl {
 
 __device__ __forceinline__ float4 load_cluster(unsigned address) {
     float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(address) : "memory");
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(address));
     return v;
 }
 template <int FORMAT, int ACT>
@@ -505,9 +506,9 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
 
     // blockIdx.x = (column tile of b * tiles of a + tile of a) * splits + rank
     const int rank = static_cast<int>(blockIdx.x % q.splits);
-    const int64_t tile = blockIdx.x / q.splits, a_tiles = (p.m + q.columns - 1) / q.columns;
-    const int64_t b0 = tile / a_tiles * kRows, a0 = tile % a_tiles * q.columns;
-    const int first = static_cast<int>(static_cast<int64_t>(q.stages) * rank / q.splits), last = static_cast<int>(static_cast<int64_t>(q.stages) * (rank + 1) / q.splits);
+    const unsigned tile = blockIdx.x / q.splits;
+    const int64_t b0 = static_cast<int64_t>(tile / q.a_tiles) * kRows, a0 = static_cast<int64_t>(tile % q.a_tiles) * q.columns;
+    const int first = static_cast<int>(static_cast<unsigned>(q.stages) * rank / q.splits), last = static_cast<int>(static_cast<unsigned>(q.stages) * (rank + 1) / q.splits);
 
     if (warp == 0) {
         int slot = 0;
@@ -559,6 +560,11 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
         }
     }
     const int height = static_cast<int>(p.m - a0 < q.columns ? p.m - a0 : q.columns);
+    const int64_t n0 = b0 + lane * 4;                  // the four rows of b that this thread finishes
+    const float alpha = __fmul_rn(p.a_scale ? *p.a_scale : 1.0f, p.b_scale ? *p.b_scale : 1.0f);
+    __align__(16) float bias[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bias[e] = p.bias && n0 + e < p.n ? load1(p.bias, p.bias_dt, n0 + e) : 0.0f;
     if (warp >= 2 && __all_sync(0xffffffffu, wait_barrier(&control.done, 0, &control.abort))) {
         // all copies into the ring and all products out of it are over: its memory takes the accumulator, 128 floats a column
         fence_after();
@@ -573,35 +579,36 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
     }
     __syncwarp();
     if (q.splits > 1) cluster_sync(); else __syncthreads();
-    {
-        // this CTA's share of the columns, four rows of b to a thread: a warp writes 128 consecutive elements of a row of the result
-        const float alpha = __fmul_rn(p.a_scale ? *p.a_scale : 1.0f, p.b_scale ? *p.b_scale : 1.0f);
-        const int share = (height + q.splits - 1) / q.splits, begin = rank * share, end = min(height, begin + share);
-        const int64_t n0 = b0 + lane * 4;
-        if (n0 < p.n && !control.abort) {
-            __align__(16) float bias[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) bias[e] = p.bias && n0 + e < p.n ? load1(p.bias, p.bias_dt, n0 + e) : 0.0f;
+    // this CTA's share of the columns, four columns x four rows of b to a thread: a warp writes 128 consecutive elements of four
+    // rows of the result, and the loads of four columns are in flight together
+    const int share = (height + q.splits * 4 - 1) / (q.splits * 4) * 4, begin = rank * share, end = min(height, begin + share);
+    if (n0 < p.n && !control.abort) {
 #pragma unroll 1
-            for (int c = begin + warp; c < end; c += kSplitThreads / 32) {
-                float4 part[kMostSplits];
+        for (int c = begin + warp * 4; c < end; c += kSplitThreads / 32 * 4) {
+            float y[4][4] = {};
+            const unsigned offset = (c * 128 + lane * 4) * 4;   // columns up to a multiple of 16 hold memory, if no values
+#pragma unroll 1
+            for (int r = 0; r < q.splits; ++r) {
+                const unsigned from = map_to_rank(buffers, q.splits > 1 ? r : cluster_rank()) + offset;
+                float4 part[4];
 #pragma unroll
-                for (int r = 0; r < kMostSplits; ++r)
-                    if (r < q.splits) part[r] = load_cluster((q.splits > 1 ? map_to_rank(buffers, r) : buffers) + (c * 128 + lane * 4) * 4);
-                float y[4] = {part[0].x, part[0].y, part[0].z, part[0].w};
+                for (int i = 0; i < 4; ++i) part[i] = load_cluster(from + i * 512);
 #pragma unroll
-                for (int r = 1; r < kMostSplits; ++r)
-                    if (r < q.splits) { y[0] += part[r].x; y[1] += part[r].y; y[2] += part[r].z; y[3] += part[r].w; }
-                finish_columns<ACT, 4>(y, bias, alpha, p.activation);
-                const int64_t at = (a0 + c) * p.n + n0;
+                for (int i = 0; i < 4; ++i) { y[i][0] += part[i].x; y[i][1] += part[i].y; y[i][2] += part[i].z; y[i][3] += part[i].w; }
+            }
+            int64_t at = (a0 + c) * p.n + n0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i, at += p.n) {
+                finish_columns<ACT, 4>(y[i], bias, alpha, p.activation);
+                if (c + i >= end) break;
                 if (p.quads && p.out_dt == VRB_BF16) {
-                    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+                    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(pack_bf16x2(y[i][0], y[i][1]), pack_bf16x2(y[i][2], y[i][3]));
                 } else if (p.quads) {
-                    *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(y[i][0], y[i][1], y[i][2], y[i][3]);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (n0 + e < p.n) store1(p.out, p.out_dt, at + e, y[e]);
+                        if (n0 + e < p.n) store1(p.out, p.out_dt, at + e, y[i][e]);
                 }
             }
         }
@@ -659,26 +666,58 @@ int launch_pair(const LinearMaps& maps, const LinearArgs& p, cudaStream_t s) {
                       sizeof(PairShared), s, maps.a, maps.b, maps.a_scales, maps.b_scales, maps.out, p);
     return after_launch("fp4_linear");
 }
-// Which kernel, and the split kernel's tile and cluster: the least of the times that a model gives, in cycles.  Measured on B200:
-// a stage of the pair kernel takes 560 (products 512), of the split kernel the time its bytes need at 72 a cycle and
-// SM; a tile costs about 1500 beyond its stages (start, drain), a split tile 2000, and another 1200 to meet in the cluster.
+// Which kernel, and the split kernel's tile and cluster: the least of the times that a model gives, in nanoseconds, fitted to
+// both kernels on B200 (back to back in a graph, within about 15 % of 130 combinations of sizes, tiles and clusters).
+// Pair kernel: 4400 + 290 a stage + 500 a tile.  Split kernel: 2600 + 260 a stage + the column work, 20 a column of the tile
+// shared by the cluster's CTAs, + 1100 to meet in a cluster; one CTA to an SM, so what does not fit at once takes turns.
 struct LinearPlan {
     int columns;   // 0: pair kernel
     int splits;
 };
+// CTAs of the split kernel at work at once for clusters of 1 to 8: processor groups are not whole multiples of a cluster
+const int* split_room() {
+    static std::atomic<int> known[64][kMostSplits + 1];
+    static thread_local int room[kMostSplits + 1];
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) device = 0;
+    for (int splits = 1; splits <= kMostSplits; ++splits) {
+        int n = known[device][splits].load(std::memory_order_relaxed);
+        if (n == 0) {
+            n = sm_count();
+            if (splits > 1) {
+                cudaLaunchConfig_t config = {};
+                config.gridDim = dim3(static_cast<unsigned>(n / splits * splits));
+                config.blockDim = dim3(kSplitThreads);
+                config.dynamicSmemBytes = 120 * 1024;   // one CTA to an SM
+                cudaLaunchAttribute attribute;
+                attribute.id = cudaLaunchAttributeClusterDimension;
+                attribute.val.clusterDim.x = static_cast<unsigned>(splits);
+                attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+                config.attrs = &attribute;
+                config.numAttrs = 1;
+                int clusters = 0;
+                const bool asked = cudaFuncSetAttribute(fp4_linear_split_kernel<VRB_NVFP4, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, 120 * 1024) == cudaSuccess &&
+                                   cudaOccupancyMaxActiveClusters(&clusters, fp4_linear_split_kernel<VRB_NVFP4, 0>, &config) == cudaSuccess && clusters > 0;
+                if (!asked) cudaGetLastError();
+                n = asked ? clusters * splits : n * 3 / 4;
+            }
+            known[device][splits].store(n, std::memory_order_relaxed);
+        }
+        room[splits] = n;
+    }
+    return room;
+}
 LinearPlan plan_linear(int64_t m, int64_t n, int stages) {
-    const int64_t sms = sm_count();
     auto ceil_div = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     LinearPlan best{0, 1};
-    const int64_t pair_tiles = ceil_div(m, kPairTile) * ceil_div(n, kPairTile);
-    int64_t least = ceil_div(pair_tiles, sms / 2 > 0 ? sms / 2 : 1) * (static_cast<int64_t>(stages) * 560 + 1500);
+    const int64_t pair_tiles = ceil_div(m, kPairTile) * ceil_div(n, kPairTile), pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1;
+    int64_t least = 4400 + ceil_div(pair_tiles, pairs) * (static_cast<int64_t>(stages) * 290 + 500);
+    const int* room = split_room();
     for (int columns = 16; columns <= 128; columns *= 2) {
-        if (columns <= 32 && m > columns) continue;   // narrower tiles than 64 would begin inside a scale word's lanes
-        const int64_t tiles = ceil_div(m, columns) * ceil_div(n, kRows), stage = (kCodeBytes + 2 * kScaleBytes + columns * kStageBytes) / 72;
+        if (columns <= 32 && m > columns) continue;   // tiles narrower than 64 would begin inside a scale word's lanes
+        const int64_t tiles = ceil_div(m, columns) * ceil_div(n, kRows);
         for (int splits = 1; splits <= kMostSplits && splits <= stages; ++splits) {
-            // clusters above 4 leave SMs of some processor groups idle
-            const int64_t room = splits > 4 ? sms * 7 / 8 : sms, ctas = tiles * splits;
-            const int64_t time = ceil_div(ctas, room) * (ceil_div(stages, splits) * stage + 2000 + (splits > 1 ? 1200 : 0));
+            const int64_t time = ceil_div(tiles * splits, room[splits]) * (2600 + ceil_div(stages, splits) * 260 + columns * 20 / splits + (splits > 1 ? 1100 : 0));
             if (time < least) { least = time; best = {columns, splits}; }
         }
         if (m <= columns) break;
@@ -693,6 +732,7 @@ int launch_split(const LinearMaps& maps, const LinearArgs& p, const LinearPlan& 
     q.columns = plan.columns;
     q.splits = plan.splits;
     q.stages = static_cast<int>((p.k + kStageElements - 1) / kStageElements);
+    q.a_tiles = static_cast<unsigned>((p.m + q.columns - 1) / q.columns);
     const int own = (q.stages + q.splits - 1) / q.splits;
     q.ring = own < kSplitRing ? own : kSplitRing;
     const size_t buffer = kCodeBytes + 2 * kScaleBytes + ((static_cast<size_t>(q.columns) * kStageBytes + 1023) & ~size_t{1023});
@@ -753,6 +793,7 @@ extern "C" int vrb_fp4_linear(int format, const void* a_codes, const void* a_sca
     VRB_REQUIRE(is_float_dtype(out_dtype) && (!bias || is_float_dtype(bias_dtype)), VRB_ERR_UNSUPPORTED, "fp4_linear: out and bias must be F32 or BF16");
     VRB_REQUIRE(rows_a > 0 && rows_b > 0 && k > 0, VRB_ERR_INVALID, "fp4_linear: rows and k must be positive");
     VRB_REQUIRE(rows_a <= INT32_MAX - 256 && rows_b <= INT32_MAX - 256 && k <= INT32_MAX - 512, VRB_ERR_INVALID, "fp4_linear: rows and k must be below 2^31 - 512");
+    VRB_REQUIRE(rows_a <= (int64_t{1} << 40) / rows_b, VRB_ERR_INVALID, "fp4_linear: the result may have at most 2^40 elements");
     VRB_REQUIRE(format == VRB_NVFP4 || (!a_tensor_scale && !b_tensor_scale), VRB_ERR_INVALID, "fp4_linear: MXFP4 has no tensor scale");
     VRB_REQUIRE(activation >= VRB_NO_ACTIVATION && activation <= VRB_RELU, VRB_ERR_INVALID, "fp4_linear: unknown activation %d", activation);
     VRB_REQUIRE(aligned16(a_codes) && aligned16(a_scales) && aligned16(b_codes) && aligned16(b_scales), VRB_ERR_INVALID,
