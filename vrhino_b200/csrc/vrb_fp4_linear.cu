@@ -456,6 +456,7 @@ constexpr int kSplitThreads = 192;
 constexpr int kSplitRing = 6;
 constexpr int kSplitColumns = 512;         // tensor memory: 128 accumulator columns, then 32 scale columns a buffer
 constexpr int kMostSplits = 8;             // portable cluster size
+constexpr size_t kSplitMostShared = kSplitRing * (2 * kCodeBytes + 2 * kScaleBytes) + 1024;
 
 struct SplitArgs {
     LinearArgs linear;
@@ -580,7 +581,7 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
     __syncwarp();
     if (q.splits > 1) cluster_sync(); else __syncthreads();
     // this CTA's share of the columns, four columns x four rows of b to a thread: a warp writes 128 consecutive elements of four
-    // rows of the result, and the loads of four columns are in flight together
+    // rows of the result, and the loads of four columns from four CTAs are in flight together
     const int share = (height + q.splits * 4 - 1) / (q.splits * 4) * 4, begin = rank * share, end = min(height, begin + share);
     if (n0 < p.n && !control.abort) {
 #pragma unroll 1
@@ -588,13 +589,20 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
             float y[4][4] = {};
             const unsigned offset = (c * 128 + lane * 4) * 4;   // columns up to a multiple of 16 hold memory, if no values
 #pragma unroll 1
-            for (int r = 0; r < q.splits; ++r) {
-                const unsigned from = map_to_rank(buffers, q.splits > 1 ? r : cluster_rank()) + offset;
-                float4 part[4];
+            for (int r = 0; r < q.splits; r += 4) {
+                float4 part[4][4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) part[i] = load_cluster(from + i * 512);
+                for (int k = 0; k < 4; ++k)
+                    if (r + k < q.splits) {
+                        const unsigned from = map_to_rank(buffers, q.splits > 1 ? r + k : cluster_rank()) + offset;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { y[i][0] += part[i].x; y[i][1] += part[i].y; y[i][2] += part[i].z; y[i][3] += part[i].w; }
+                        for (int i = 0; i < 4; ++i) part[k][i] = load_cluster(from + i * 512);
+                    }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (r + k < q.splits)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) { y[i][0] += part[k][i].x; y[i][1] += part[k][i].y; y[i][2] += part[k][i].z; y[i][3] += part[k][i].w; }
             }
             int64_t at = (a0 + c) * p.n + n0;
 #pragma unroll
@@ -652,6 +660,19 @@ bool encode_scales(CUtensorMap* map, int format, const void* scales, int64_t row
                      CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
+// Lets a kernel have `bytes` of dynamic shared memory; asked once per device (`done`: a bit for each).
+template <typename Kernel>
+int allow_shared(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done) {
+    int device = 0;
+    const bool known = cudaGetDevice(&device) == cudaSuccess && device >= 0 && device < 64;
+    const uint64_t bit = known ? uint64_t{1} << device : 0;
+    if (done.load(std::memory_order_acquire) & bit) return VRB_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    VRB_REQUIRE(e == cudaSuccess, VRB_ERR_CUDA, "CUDA error: %s (fp4_linear)", cudaGetErrorString(e));
+    done.fetch_or(bit, std::memory_order_release);
+    return VRB_OK;
+}
+
 struct LinearMaps {
     CUtensorMap a, b, a_scales, b_scales, out;
 };
@@ -659,17 +680,17 @@ struct LinearMaps {
 template <int FORMAT, int ACT, int OUT>
 int launch_pair(const LinearMaps& maps, const LinearArgs& p, cudaStream_t s) {
     static_assert(sizeof(PairShared) <= 227 * 1024, "ring does not fit shared memory");
-    const cudaError_t e = cudaFuncSetAttribute(fp4_linear_pair_kernel<FORMAT, ACT, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(PairShared));
-    VRB_REQUIRE(e == cudaSuccess, VRB_ERR_CUDA, "CUDA error: %s (fp4_linear)", cudaGetErrorString(e));
+    static std::atomic<uint64_t> allowed{0};
+    if (int rc = allow_shared(fp4_linear_pair_kernel<FORMAT, ACT, OUT>, sizeof(PairShared), allowed)) return rc;
     const int64_t tiles = ((p.m + kPairTile - 1) / kPairTile) * ((p.n + kPairTile - 1) / kPairTile), pairs = sm_count() / 2;
     launch_overlapped(fp4_linear_pair_kernel<FORMAT, ACT, OUT>, dim3(static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs))), dim3(kPairThreads),
                       sizeof(PairShared), s, maps.a, maps.b, maps.a_scales, maps.b_scales, maps.out, p);
     return after_launch("fp4_linear");
 }
 // Which kernel, and the split kernel's tile and cluster: the least of the times that a model gives, in nanoseconds, fitted to
-// both kernels on B200 (back to back in a graph, within about 15 % of 130 combinations of sizes, tiles and clusters).
-// Pair kernel: 4400 + 290 a stage + 500 a tile.  Split kernel: 2600 + 260 a stage + the column work, 20 a column of the tile
-// shared by the cluster's CTAs, + 1100 to meet in a cluster; one CTA to an SM, so what does not fit at once takes turns.
+// both kernels on B200 (back to back in a graph; the choice is within 3 % of the best on 24 shapes between 1 x 512 x 512
+// and 4000 x 6000 x 30720).  Pair kernel: 4300 + 500 a tile + 290 a stage.  Split kernel: 2300 + 19 a column
+// of the tile + 265 a stage, and 800 + 130 a CTA to meet in a cluster; one CTA to an SM, what does not fit at once takes turns.
 struct LinearPlan {
     int columns;   // 0: pair kernel
     int splits;
@@ -696,7 +717,7 @@ const int* split_room() {
                 config.attrs = &attribute;
                 config.numAttrs = 1;
                 int clusters = 0;
-                const bool asked = cudaFuncSetAttribute(fp4_linear_split_kernel<VRB_NVFP4, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, 120 * 1024) == cudaSuccess &&
+                const bool asked = cudaFuncSetAttribute(fp4_linear_split_kernel<VRB_NVFP4, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSplitMostShared) == cudaSuccess &&
                                    cudaOccupancyMaxActiveClusters(&clusters, fp4_linear_split_kernel<VRB_NVFP4, 0>, &config) == cudaSuccess && clusters > 0;
                 if (!asked) cudaGetLastError();
                 n = asked ? clusters * splits : n * 3 / 4;
@@ -711,13 +732,13 @@ LinearPlan plan_linear(int64_t m, int64_t n, int stages) {
     auto ceil_div = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     LinearPlan best{0, 1};
     const int64_t pair_tiles = ceil_div(m, kPairTile) * ceil_div(n, kPairTile), pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1;
-    int64_t least = 4400 + ceil_div(pair_tiles, pairs) * (static_cast<int64_t>(stages) * 290 + 500);
+    int64_t least = 4300 + ceil_div(pair_tiles, pairs) * (static_cast<int64_t>(stages) * 290 + 500);
     const int* room = split_room();
     for (int columns = 16; columns <= 128; columns *= 2) {
         if (columns <= 32 && m > columns) continue;   // tiles narrower than 64 would begin inside a scale word's lanes
         const int64_t tiles = ceil_div(m, columns) * ceil_div(n, kRows);
         for (int splits = 1; splits <= kMostSplits && splits <= stages; ++splits) {
-            const int64_t time = ceil_div(tiles * splits, room[splits]) * (2600 + ceil_div(stages, splits) * 260 + columns * 20 / splits + (splits > 1 ? 1100 : 0));
+            const int64_t time = ceil_div(tiles * splits, room[splits]) * (2300 + columns * 19 + ceil_div(stages, splits) * 265 + (splits > 1 ? 800 + 130 * splits : 0));
             if (time < least) { least = time; best = {columns, splits}; }
         }
         if (m <= columns) break;
@@ -739,10 +760,9 @@ int launch_split(const LinearMaps& maps, const LinearArgs& p, const LinearPlan& 
     size_t bytes = q.ring * buffer;
     if (bytes < static_cast<size_t>(q.columns) * 512) bytes = static_cast<size_t>(q.columns) * 512;
     bytes += 1024;
-    static_assert(kSplitRing * (2 * kCodeBytes + 2 * kScaleBytes) + 1024 + sizeof(SplitControl) <= 227 * 1024, "ring does not fit shared memory");
-    cudaError_t e = cudaFuncSetAttribute(fp4_linear_split_kernel<FORMAT, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         kSplitRing * (2 * kCodeBytes + 2 * kScaleBytes) + 1024);
-    VRB_REQUIRE(e == cudaSuccess, VRB_ERR_CUDA, "CUDA error: %s (fp4_linear)", cudaGetErrorString(e));
+    static_assert(kSplitMostShared + sizeof(SplitControl) <= 227 * 1024, "ring does not fit shared memory");
+    static std::atomic<uint64_t> allowed{0};
+    if (int rc = allow_shared(fp4_linear_split_kernel<FORMAT, ACT>, kSplitMostShared, allowed)) return rc;
     const int64_t tiles = ((p.m + q.columns - 1) / q.columns) * ((p.n + kRows - 1) / kRows);
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(static_cast<unsigned>(tiles * q.splits));

@@ -15,7 +15,9 @@ Every call goes to the CUDA library; nothing here computes on the CPU or through
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import math
 from dataclasses import dataclass, field
 
 import torch
@@ -47,6 +49,36 @@ def _code(t_or_dtype):
 
 def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+_functions = {}
+
+
+def _launch(name, device, *args):
+    """The entry point `name` on `device`, on that device's current stream (its last argument), whichever device is current.
+    Plain integers go through ctypes: the small operators cost as much on the host as on the GPU."""
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(_lib.load(), name)
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status)
+
+
+def _address(t, device):
+    """Device address of an optional operand that has to lie on `device`, contiguous."""
+    if t is None:
+        return None
+    if t.device != device:
+        raise VrbError("Tensors must be on one device")
+    if not t.is_contiguous():
+        raise VrbError("Tensor must be contiguous")
+    return t.data_ptr()
 
 
 def _shape(t):
@@ -94,10 +126,35 @@ class Fp4Tensor:
 
     @property
     def rows(self):
-        rows = 1
-        for d in self.shape[:-1]:
-            rows *= d
-        return rows
+        return math.prod(self.shape[:-1])
+
+
+_FP4_BLOCK = {NVFP4: 16, MXFP4: 32}
+_here = contextlib.nullcontext()
+
+
+def _fp4_row_bytes(k):
+    """vrb_fp4_row_bytes"""
+    return (k + 31) // 32 * 16
+
+
+def _fp4_scale_bytes(format, rows, k):
+    """vrb_fp4_scale_bytes"""
+    span = 4 * _FP4_BLOCK[format]
+    return (rows + 127) // 128 * ((k + span - 1) // span) * 512
+
+
+def _fp4_addresses(q, rows, k, device):
+    """Device addresses of a packed operand's parts after a check of what they have to hold."""
+    codes, scales, scale = q.codes, q.scales, q.tensor_scale
+    if q.format not in _FP4_BLOCK or rows <= 0 or k <= 0 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or \
+            tuple(codes.shape) != (rows, _fp4_row_bytes(k)) or scales.numel() != _fp4_scale_bytes(q.format, rows, k):
+        raise VrbError("fp4 operand: codes or scales do not match the shape and format")
+    if scale is not None and (scale.dtype != F32 or scale.numel() != 1 or scale.device != device):
+        raise VrbError("fp4 tensor scale must be one F32 on the operand's device")
+    if not codes.is_cuda:
+        raise VrbError("Tensor must be device-resident")
+    return _address(codes, device), _address(scales, device), None if scale is None else scale.data_ptr()
 
 
 class HostScalar:
@@ -589,82 +646,76 @@ class B200Backend:
         for name, t in (("weight", weight), ("bias", bias)):
             if t is not None and t.numel() != channels:
                 raise VrbError(f"group norm {name} mismatch")
-        out = _result(out, x.shape, x.dtype, x.device)
+        device = x.device
+        out = _result(out, x.shape, dtype, device)
         if x.numel() == 0:
             return out
+        code = _CODE[dtype]
         spatial = x.numel() // (batch * channels)
-        need = _lib.load().vrb_group_norm_channels_last_workspace_bytes(_code(x), batch, spatial, channels, groups)
+        with torch.cuda.device(device) if device.index != torch._C._cuda_getDevice() else _here:
+            need = _lib.load().vrb_group_norm_channels_last_workspace_bytes(code, batch, spatial, channels, groups)
         # scratch of this call alone: torch's allocator keeps it from other streams and other captured graphs
-        scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-        call("vrb_group_norm_channels_last", _ptr(x), _code(x), _ptr(weight), _code(weight) if weight is not None else 0,
-             _ptr(bias), _code(bias) if bias is not None else 0, _ptr(out), batch, spatial, channels, groups,
-             ctypes.c_float(eps), _lib.NO_ACTIVATION if activation is None else int(activation), _ptr(scratch), need, _stream())
+        scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        _launch("vrb_group_norm_channels_last", device, x.data_ptr(), code, _address(weight, device), 0 if weight is None else _code(weight),
+                _address(bias, device), 0 if bias is None else _code(bias), out.data_ptr(), batch, spatial, channels, groups, eps,
+                _lib.NO_ACTIVATION if activation is None else int(activation), scratch.data_ptr() if need else None, need)
         return out
 
     # ---- microscaled 4-bit operands (include/vrb.h) ----
     def fp4_tensor_scale(self, raw, out=None):
         """The NVFP4 tensor scale of x as a device F32 [1]: max(|x|) / 2688."""
-        x = _dense(self.copy_to_device(raw, self._dtype_of(raw)))
+        dtype = self._dtype_of(raw)
+        x = _dense(self.copy_to_device(raw, dtype))
         out = _result(out, (1,), F32, x.device)
-        call("vrb_fp4_tensor_scale", _ptr(x), _code(x), x.numel(), _ptr(out), _stream())
+        _launch("vrb_fp4_tensor_scale", x.device, x.data_ptr(), _CODE[dtype], x.numel(), out.data_ptr())
         return out
 
     def fp4_quantize(self, raw, format=NVFP4, tensor_scale=None, out=None):
         """Packs x [..., k] into 4 bits an element with a scale per block of a row; NVFP4 takes a device F32 tensor scale
         (fp4_tensor_scale, or one calibrated beforehand; None = 1)."""
-        x = _dense(self.copy_to_device(raw, self._dtype_of(raw)))
-        if x.dim() < 1 or x.numel() == 0:
+        dtype = self._dtype_of(raw)
+        x = _dense(self.copy_to_device(raw, dtype))
+        count, device = x.numel(), x.device
+        if x.dim() < 1 or count == 0:
             raise VrbError("fp4_quantize: rows and k must be positive")
-        if format not in (NVFP4, MXFP4):
+        if format not in _FP4_BLOCK:
             raise VrbError(f"fp4_quantize: unknown 4-bit format {format}")
-        k = x.shape[-1]
-        rows = x.numel() // k
-        lib = _lib.load()
-        code_shape, scale_bytes = (rows, lib.vrb_fp4_row_bytes(k)), lib.vrb_fp4_scale_bytes(format, rows, k)
-        if out is not None and (out.format != format or out.tensor_scale is not tensor_scale or tuple(out.shape) != tuple(x.shape)):
+        shape = tuple(x.shape)
+        k = shape[-1]
+        rows = count // k
+        if out is None:
+            out = Fp4Tensor(torch.empty((rows, _fp4_row_bytes(k)), dtype=torch.uint8, device=device),
+                            torch.empty(_fp4_scale_bytes(format, rows, k), dtype=torch.uint8, device=device), tensor_scale, format, shape)
+        elif out.format != format or out.tensor_scale is not tensor_scale or tuple(out.shape) != shape or out.codes.device != device:
             raise VrbError("output buffer does not match the result's shape, dtype or device")
-        codes = _result(None if out is None else out.codes, code_shape, torch.uint8, x.device)
-        scales = _result(None if out is None else out.scales, (scale_bytes,), torch.uint8, x.device)
-        self._fp4_scale(tensor_scale, x.device)
-        call("vrb_fp4_quantize", format, _ptr(x), _code(x), _ptr(tensor_scale), _ptr(codes), _ptr(scales), rows, k, _stream())
-        return out if out is not None else Fp4Tensor(codes, scales, tensor_scale, format, tuple(x.shape))
-
-    @staticmethod
-    def _fp4_scale(tensor_scale, device):
-        if tensor_scale is not None and (tensor_scale.dtype != F32 or tensor_scale.numel() != 1 or tensor_scale.device != device):
-            raise VrbError("fp4 tensor scale must be one F32 on the operand's device")
-
-    def _fp4_operand(self, q):
-        lib = _lib.load()
-        rows, k = q.rows, q.k
-        if rows <= 0 or k <= 0 or tuple(q.codes.shape) != (rows, lib.vrb_fp4_row_bytes(k)) or q.codes.dtype != torch.uint8 or \
-                q.scales.dtype != torch.uint8 or q.scales.numel() != lib.vrb_fp4_scale_bytes(q.format, rows, k):
-            raise VrbError("fp4 operand: codes or scales do not match the shape and format")
-        _dense(q.codes), _dense(q.scales)
-        self._fp4_scale(q.tensor_scale, q.codes.device)
-        return rows, k
+        codes, scales, scale = _fp4_addresses(out, rows, k, device)
+        _launch("vrb_fp4_quantize", device, format, x.data_ptr(), _CODE[dtype], scale, codes, scales, rows, k)
+        return out
 
     def fp4_dequantize(self, q, dtype=BF16, out=None):
         """The values a packed operand stands for, in `dtype` (the 4-bit sibling of dequantize)."""
-        rows, k = self._fp4_operand(q)
-        out = _result(out, q.shape, dtype, q.codes.device)
-        call("vrb_fp4_dequantize", q.format, _ptr(q.codes), _ptr(q.scales), _ptr(q.tensor_scale), _ptr(out), _code(dtype), rows, k, _stream())
+        rows, k, device = q.rows, q.k, q.codes.device
+        codes, scales, scale = _fp4_addresses(q, rows, k, device)
+        out = _result(out, q.shape, dtype, device)
+        _launch("vrb_fp4_dequantize", device, q.format, codes, scales, scale, out.data_ptr(), _code(dtype), rows, k)
         return out
 
     def fp4_linear(self, x, weight, bias=None, activation=None, dtype=BF16, out=None):
         """activation(x weight^T + bias) over packed operands x [..., k] and weight [n, k] of one format -> [..., n] in
         `dtype`, accumulated in F32.  dtype F32 without bias and activation is the accumulation that linear_output and
         its merged forms read."""
-        m, k = self._fp4_operand(x)
-        n, kw = self._fp4_operand(weight)
-        if x.format != weight.format or k != kw or len(weight.shape) != 2:
+        m, k, device = x.rows, x.k, x.codes.device
+        if x.format != weight.format or len(weight.shape) != 2 or weight.shape[1] != k:
             raise VrbError("fp4_linear: operands differ in format or width")
-        if bias is not None and (_dense(bias).numel() != n):
+        n = weight.shape[0]
+        a_codes, a_scales, a_scale = _fp4_addresses(x, m, k, device)
+        b_codes, b_scales, b_scale = _fp4_addresses(weight, n, k, device)
+        if bias is not None and bias.numel() != n:
             raise VrbError("linear bias mismatch")
-        out = _result(out, tuple(x.shape[:-1]) + (n,), dtype, x.codes.device)
-        call("vrb_fp4_linear", x.format, _ptr(x.codes), _ptr(x.scales), _ptr(x.tensor_scale), m, _ptr(weight.codes), _ptr(weight.scales),
-             _ptr(weight.tensor_scale), n, k, _ptr(bias), _code(bias) if bias is not None else 0,
-             _lib.NO_ACTIVATION if activation is None else int(activation), _ptr(out), _code(dtype), _stream())
+        shape = tuple(x.shape[:-1]) + (n,)
+        out = torch.empty(shape, dtype=dtype, device=device) if out is None else _result(out, shape, dtype, device)
+        _launch("vrb_fp4_linear", device, x.format, a_codes, a_scales, a_scale, m, b_codes, b_scales, b_scale, n, k, _address(bias, device),
+                0 if bias is None else _code(bias), _lib.NO_ACTIVATION if activation is None else int(activation), out.data_ptr(), _code(dtype))
         return out
 
 
