@@ -6,20 +6,24 @@
 // The bound is HBM: x is read for the statistics and again for the result, which is written once (the reference would
 // add two permutes).  A thread owns V consecutive channels (16 bytes where the layout allows) of every rpp-th row,
 // so the affine terms and the group look-up are per thread, not per element, and consecutive threads read consecutive
-// bytes of a row.
-//   1. gcl_partial   per thread F32 sums of (x - K) and (x - K)^2 per channel over runs of kRun rows, K the run's
-//                    first value (an offset common to the channel cancels exactly), rebuilt in double:
-//                    S = s1 + n K, Q = s2 + K (2 s1 + n K); the threads of a group are added in a fixed order
-//   2. gcl_finalize  adds the CTAs' partials of a (batch entry, group) in a fixed order; mean, rsqrt(var + eps)
-//   3. gcl_apply     sweeps the rows backwards, so that it starts with what the statistics pass left in L2
+// bytes of a row.  Statistics everywhere: per thread and channel F32 sums of (x - K) and (x - K)^2 over at most kRun rows, K
+// the first value of the run (an offset common to the channel cancels exactly), rebuilt in double: S = s1 + n K,
+// Q = s2 + K (2 s1 + n K); threads, CTAs and clusters are added in a fixed order.
+//   Feature maps that fit the registers of one cluster per slab of channels: gcl_cluster reads x once, keeps it, adds the sums
+//   over distributed shared memory and writes the result: one launch.
+//   Others: 1. gcl_partial   a CTA's sums per (batch entry, group)
+//           2. gcl_finalize  only for many groups: adds the CTAs' sums once, where adding them in every CTA of 3. would cost more
+//           3. gcl_apply     sweeps the rows backwards, so that it starts with what the statistics pass left in L2
 #include "vrb_common.cuh"
 
 namespace vrb {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;      // of the passes
+constexpr int kClusterThreads = 256;
 constexpr int kRun = 32;           // rows of a thread between two rebuilds in double
-constexpr int kSplitsPerSm = 2;    // CTAs of the statistics pass per SM
+constexpr int kClusterGroups = 128;// groups of a cluster's slab, at most
+constexpr int kInlineGroups = 64;  // groups up to which gcl_apply adds the CTAs' sums itself
 
 struct GclGeom {
     int64_t batch, spatial;
@@ -27,20 +31,34 @@ struct GclGeom {
     int vectors;                   // channels / V
     int slab;                      // vectors a CTA covers at a time (<= kThreads)
     int rpp;                       // rows a CTA covers at a time
-    int splits;                    // CTAs per batch entry (statistics)
+    int splits;                    // CTAs of the statistics pass per batch entry
+    int cluster;                   // CTAs of a cluster of gcl_cluster
+    double share;                  // 1 / elements of a group
 };
 
+__device__ __forceinline__ unsigned cluster_rank() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory"); }
+// the double at `local` in the shared memory of the cluster's CTA `rank`
+__device__ __forceinline__ double load_cluster(const double* local, unsigned rank) {
+    double v;
+    asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f64 %0, [a];\n\t}"
+                 : "=d"(v) : "r"(static_cast<unsigned>(__cvta_generic_to_shared(local))), "r"(rank) : "memory");
+    return v;
+}
+
+// V elements as the 32-bit words they are loaded as (an array of halves would be moved half by half)
 template <typename T, int V>
-struct Vec;
-template <int V>
-struct Vec<uint16_t, V> {
-    uint16_t raw[V];
-    __device__ __forceinline__ float get(int e) const { return bf16_bits_to_float(raw[e]); }
-};
-template <int V>
-struct Vec<float, V> {
-    float raw[V];
-    __device__ __forceinline__ float get(int e) const { return raw[e]; }
+struct Vec {
+    static constexpr int kBytes = static_cast<int>(sizeof(T)) * V, kWords = (kBytes + 3) / 4;
+    uint32_t word[kWords];
+    __device__ __forceinline__ float get(int e) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(word[e]);
+        else return __uint_as_float(e & 1 ? word[e / 2] & 0xffff0000u : word[e / 2] << 16);
+    }
 };
 template <int BYTES> struct Word;
 template <> struct Word<16> { using type = uint4; };
@@ -48,39 +66,29 @@ template <> struct Word<8> { using type = uint2; };
 template <> struct Word<4> { using type = uint32_t; };
 template <> struct Word<2> { using type = uint16_t; };
 
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> load_vec(const T* p) {
-    using W = typename Word<sizeof(T) * V>::type;
-    const W w = __ldcs(reinterpret_cast<const W*>(p));
+template <bool STREAM, typename T, int V>
+__device__ __forceinline__ Vec<T, V> load_vec(const T* p) {   // STREAM: not worth keeping in L2
+    using W = typename Word<Vec<T, V>::kBytes>::type;
+    const W w = STREAM ? __ldcs(reinterpret_cast<const W*>(p)) : *reinterpret_cast<const W*>(p);
     Vec<T, V> r;
-    *reinterpret_cast<W*>(r.raw) = w;
-    return r;
-}
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> load_vec_keep(const T* p) {   // default policy: the line should stay in L2
-    using W = typename Word<sizeof(T) * V>::type;
-    const W w = *reinterpret_cast<const W*>(p);
-    Vec<T, V> r;
-    *reinterpret_cast<W*>(r.raw) = w;
+    if constexpr (sizeof(W) == 16) { r.word[0] = w.x; r.word[1] = w.y; r.word[2] = w.z; r.word[3] = w.w; }
+    else if constexpr (sizeof(W) == 8) { r.word[0] = w.x; r.word[1] = w.y; }
+    else r.word[0] = w;
     return r;
 }
 template <int V>
 __device__ __forceinline__ void store_vec(uint16_t* p, const float (&v)[V]) {
-    using W = typename Word<2 * V>::type;
-    union { W w; uint16_t h[V]; uint32_t d[V / 2 > 0 ? V / 2 : 1]; } r;
-    if constexpr (V == 1) r.h[0] = static_cast<uint16_t>(float_to_bf16_bits(v[0]));
-    else
-#pragma unroll
-        for (int e = 0; e < V; e += 2) r.d[e / 2] = pack_bf16x2(v[e], v[e + 1]);
-    __stcs(reinterpret_cast<W*>(p), r.w);
+    if constexpr (V == 8)
+        __stcs(reinterpret_cast<uint4*>(p), make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])));
+    else if constexpr (V == 4) __stcs(reinterpret_cast<uint2*>(p), make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])));
+    else if constexpr (V == 2) __stcs(reinterpret_cast<uint32_t*>(p), pack_bf16x2(v[0], v[1]));
+    else __stcs(p, static_cast<uint16_t>(float_to_bf16_bits(v[0])));
 }
 template <int V>
 __device__ __forceinline__ void store_vec(float* p, const float (&v)[V]) {
-    using W = typename Word<4 * V>::type;
-    union { W w; float f[V]; } r;
-#pragma unroll
-    for (int e = 0; e < V; ++e) r.f[e] = v[e];
-    __stcs(reinterpret_cast<W*>(p), r.w);
+    if constexpr (V == 4) __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+    else if constexpr (V == 2) __stcs(reinterpret_cast<float2*>(p), make_float2(v[0], v[1]));
+    else __stcs(p, v[0]);
 }
 
 // The activation on an F32 value that is rounded once afterwards.  SiLU and GELU-tanh go through one exponential and
@@ -97,137 +105,223 @@ __device__ __forceinline__ float activate(float y, int kind) {
     return activation_value(kind, y);
 }
 
-// partial[((b * splits + split) * groups + g) * 2 + {0, 1}] = {sum x, sum x^2} over the CTA's rows
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads, V >= 4 ? 2 : 4) gcl_partial_kernel(const T* x, double* __restrict__ partial, GclGeom g) {
-    __shared__ double sums[2][kThreads * V];
+// Sums of a thread's V channels over a run, and what has been rebuilt from earlier runs.  WHOLE: the V channels lie in one group
+// and share the double sums.
+template <typename T, int V, bool WHOLE>
+struct Sums {
+    static constexpr int D = WHOLE ? 1 : V;
+    double S[D], Q[D];
+    float K[V], s1[V], s2[V];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int e = 0; e < D; ++e) S[e] = Q[e] = 0.0;
+    }
+    __device__ __forceinline__ void begin(const Vec<T, V>& v) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) { K[e] = v.get(e); s1[e] = s2[e] = 0.0f; }
+    }
+    __device__ __forceinline__ void add(const Vec<T, V>& v) {
+        if constexpr (V > 1) {
+#pragma unroll
+            for (int e = 0; e < V; e += 2) {
+                const unsigned long long d = sub_f32x2(pack_f32x2(v.get(e), v.get(e + 1)), pack_f32x2(K[e], K[e + 1]));
+                unpack_f32x2(add_f32x2(pack_f32x2(s1[e], s1[e + 1]), d), s1[e], s1[e + 1]);
+                unpack_f32x2(fma_f32x2(d, d, pack_f32x2(s2[e], s2[e + 1])), s2[e], s2[e + 1]);
+            }
+        } else {
+            const float d = v.get(0) - K[0];
+            s1[0] += d;
+            s2[0] = fmaf(d, d, s2[0]);
+        }
+    }
+    __device__ __forceinline__ void rebuild(int n) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const double k = K[e], nk = n * k;
+            S[WHOLE ? 0 : e] += s1[e] + nk;
+            Q[WHOLE ? 0 : e] += s2[e] + k * (2.0 * s1[e] + nk);
+        }
+    }
+};
+
+// Adds the CTA's sums of one slab per group: a warp to a group, lanes strided over (row, D-channel entry), a fixed tree.  Every
+// group's {S, Q} goes to `take(group - first group of the slab, S, Q)` on lane 0.
+template <int THREADS, int D, int V, typename Take>
+__device__ __forceinline__ void add_groups(double (&sums)[2][THREADS * D], const GclGeom& g, int slab0, int slab, Take take) {
+    const int lane = threadIdx.x & 31, c_begin = slab0 * V, c_end = c_begin + slab * V, first = c_begin / g.per;
+    constexpr int E = V / D;   // channels of an entry
+    for (int group = first + (threadIdx.x >> 5); group * g.per < c_end; group += THREADS / 32) {
+        const int from = (max(group * g.per, c_begin) - c_begin) / E, width = (min((group + 1) * g.per, c_end) - c_begin) / E - from;
+        double s = 0.0, q = 0.0;
+        int r = 0, at = lane;
+        while (at >= width && r < g.rpp) { at -= width; ++r; }
+        while (r < g.rpp) {
+            const int i = r * g.slab * D + from + at;
+            s += sums[0][i];
+            q += sums[1][i];
+            at += 32;
+            while (at >= width && r < g.rpp) { at -= width; ++r; }
+        }
+        for (int offset = 16; offset > 0; offset >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, offset);
+            q += __shfl_xor_sync(0xffffffffu, q, offset);
+        }
+        if (lane == 0) take(group - first, s, q);
+    }
+}
+// {mean, rsqrt(var + eps)}; share = 1 / n.  Products in double, where the squared mean cancels; no double division or square
+// root, which took a third of the normalise pass on 25 MB.
+__device__ __forceinline__ float2 moments_to_stats(double s, double q, double share, float eps) {
+    const double mean = s * share;
+    float var = static_cast<float>(q * share - mean * mean);
+    if (var < 0.0f) var = 0.0f;                        // a NaN stays
+    return make_float2(static_cast<float>(mean), rsqrtf(var + eps));
+}
+
+// partial[((b * splits + split) * groups + g) * 2 + {0, 1}] = {sum x, sum x^2} over the CTA's rows.  One CTA to an SM.
+template <typename T, int V, bool WHOLE>
+__global__ void __launch_bounds__(kThreads, 1) gcl_partial_kernel(const T* x, double* __restrict__ partial, GclGeom g) {
+    using Acc = Sums<T, V, WHOLE>;
+    __shared__ double sums[2][kThreads * Acc::D];
     pdl_wait();
     const int b = blockIdx.x / g.splits, split = blockIdx.x - b * g.splits;
     const int lane_vector = threadIdx.x % g.slab, lane_row = threadIdx.x / g.slab;
     double* out = partial + static_cast<int64_t>(blockIdx.x) * g.groups * 2;
     for (int slab0 = 0; slab0 < g.vectors; slab0 += g.slab) {
         const int slab = min(g.slab, g.vectors - slab0);
-        double S[V], Q[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) S[e] = Q[e] = 0.0;
+        Acc acc;
+        acc.clear();
         if (lane_row < g.rpp && lane_vector < slab) {
-            const int64_t step = static_cast<int64_t>(g.splits) * g.rpp;
-            int64_t row = static_cast<int64_t>(split) * g.rpp + lane_row;
+            constexpr int U = WHOLE && sizeof(T) * V == 16 ? 8 : 4;
+            const int64_t step = static_cast<int64_t>(g.splits) * g.rpp, p_step = step * g.channels;
+            const int64_t row = static_cast<int64_t>(split) * g.rpp + lane_row;
             const T* p = x + (static_cast<int64_t>(b) * g.spatial + row) * g.channels + (slab0 + lane_vector) * V;
-            const int64_t p_step = step * g.channels;
-            while (row < g.spatial) {
-                float K[V], s1[V], s2[V];
-                int n = 0;
+            int64_t left = row < g.spatial ? (g.spatial - 1 - row) / step + 1 : 0;   // rows of this thread from p on
+            // U rows at a time, the next U on their way while these are added
+            Vec<T, V> now[U], next[U];
 #pragma unroll
-                for (int e = 0; e < V; ++e) s1[e] = s2[e] = 0.0f;
-                for (; n < kRun && row < g.spatial; ) {
-                    constexpr int U = 4;
-                    Vec<T, V> v[U];
-                    int have = 0;
+            for (int u = 0; u < U; ++u)
+                if (u < left) now[u] = load_vec<false, T, V>(p + u * p_step);
+            int run = 0;
+            for (; left > 0; left -= U) {
+                p += U * p_step;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (U + u < left) next[u] = load_vec<false, T, V>(p + u * p_step);
+                if (run == 0) acc.begin(now[0]);
+                if (left >= U) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) acc.add(now[u]);
+                } else {
 #pragma unroll
                     for (int u = 0; u < U; ++u)
-                        if (row + u * step < g.spatial) { v[u] = load_vec_keep<T, V>(p + u * p_step); have = u + 1; }
-                    if (n == 0)
-#pragma unroll
-                        for (int e = 0; e < V; ++e) K[e] = v[0].get(e);
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-                        if (u < have)
-#pragma unroll
-                            for (int e = 0; e < V; ++e) {
-                                const float d = v[u].get(e) - K[e];
-                                s1[e] += d;
-                                s2[e] = fmaf(d, d, s2[e]);
-                            }
-                    n += have;
-                    row += U * step;
-                    p += U * p_step;
+                        if (u < left) acc.add(now[u]);
+                }
+                run += left < U ? static_cast<int>(left) : U;
+                if (run >= kRun || left <= U) {
+                    acc.rebuild(run);
+                    run = 0;
                 }
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const double k = K[e], nk = n * k;
-                    S[e] += s1[e] + nk;
-                    Q[e] += s2[e] + k * (2.0 * s1[e] + nk);
-                }
+                for (int u = 0; u < U; ++u) now[u] = next[u];
             }
         }
         if (slab0) __syncthreads();
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            sums[0][threadIdx.x * V + e] = S[e];
-            sums[1][threadIdx.x * V + e] = Q[e];
+        for (int e = 0; e < Acc::D; ++e) {
+            sums[0][threadIdx.x * Acc::D + e] = acc.S[e];
+            sums[1][threadIdx.x * Acc::D + e] = acc.Q[e];
         }
         __syncthreads();
-        // one warp per group: the slab's channels of the group, over the CTA's rows, strided over the lanes
-        const int c_begin = slab0 * V, c_end = c_begin + slab * V;
-        const int lane = threadIdx.x & 31;
-        for (int group = c_begin / g.per + (threadIdx.x >> 5); group * g.per < c_end; group += kThreads / 32) {
-            const int from = max(group * g.per, c_begin) - c_begin, width = min((group + 1) * g.per, c_end) - c_begin - from;
-            double s = 0.0, q = 0.0;
-            for (int i = lane; i < width * g.rpp; i += 32) {
-                const int r = i / width, at = r * g.slab * V + from + (i - r * width);
-                s += sums[0][at];
-                q += sums[1][at];
-            }
-            for (int offset = 16; offset > 0; offset >>= 1) {
-                s += __shfl_xor_sync(0xffffffffu, s, offset);
-                q += __shfl_xor_sync(0xffffffffu, q, offset);
-            }
-            if (lane == 0) {
-                if (group * g.per < c_begin) { s += out[group * 2]; q += out[group * 2 + 1]; }   // begun in an earlier slab
-                out[group * 2] = s;
-                out[group * 2 + 1] = q;
-            }
-        }
+        const int first = slab0 * V / g.per;
+        add_groups<kThreads, Acc::D, V>(sums, g, slab0, slab, [&](int group, double s, double q) {
+            double* o = out + (first + group) * 2;
+            if ((first + group) * g.per < slab0 * V) { s += o[0]; q += o[1]; }   // begun in an earlier slab
+            o[0] = s;
+            o[1] = q;
+        });
         __syncthreads();
     }
 }
 
-// stats[(b * groups + g) * 2 + {0, 1}] = {mean, rsqrt(var + eps)}; one warp per (batch entry, group)
-__global__ void __launch_bounds__(128) gcl_finalize_kernel(const double* __restrict__ partial, float* __restrict__ stats, GclGeom g, float eps) {
+// {mean, rsqrt(var + eps)} of groups [first, first + count) of a batch entry from the CTAs' sums, count <= THREADS: neighbouring
+// threads read neighbouring groups, THREADS / count of them share a group's clusters; all threads of the CTA together.
+template <int THREADS, typename Take>
+__device__ __forceinline__ void collect_groups(const double* partial, int64_t b, int first, int count, const GclGeom& g, float eps, Take take) {
+    __shared__ double2 parts[THREADS];
+    const int shares = THREADS / count, group = threadIdx.x % count, share = threadIdx.x / count;
+    double2 sum = make_double2(0.0, 0.0);
+    if (share < shares) {
+        const double2* p = reinterpret_cast<const double2*>(partial) + b * g.splits * g.groups + first + group;
+#pragma unroll 8
+        for (int i = share; i < g.splits; i += shares) {
+            const double2 v = p[static_cast<int64_t>(i) * g.groups];
+            sum.x += v.x;
+            sum.y += v.y;
+        }
+    }
+    parts[threadIdx.x] = sum;
+    __syncthreads();
+    if (threadIdx.x < count) {
+        for (int i = 1; i < shares; ++i) {
+            sum.x += parts[i * count + group].x;
+            sum.y += parts[i * count + group].y;
+        }
+        take(group, moments_to_stats(sum.x, sum.y, g.share, eps));
+    }
+    __syncthreads();
+}
+// stats[b * groups + g] = {mean, rsqrt(var + eps)}; a CTA to 32 groups
+constexpr int kFinalizeGroups = 32;
+__global__ void __launch_bounds__(kThreads) gcl_finalize_kernel(const double* __restrict__ partial, float2* __restrict__ stats, GclGeom g, float eps) {
     pdl_wait();
-    const int64_t unit = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-    const int lane = threadIdx.x & 31;
-    if (unit >= g.batch * g.groups) return;
-    const int64_t b = unit / g.groups;
-    const int group = static_cast<int>(unit - b * g.groups);
-    double s = 0.0, q = 0.0;
-    for (int i = lane; i < g.splits; i += 32) {
-        const double* p = partial + ((b * g.splits + i) * g.groups + group) * 2;
-        s += p[0];
-        q += p[1];
+    const int chunks = (g.groups + kFinalizeGroups - 1) / kFinalizeGroups;
+    const int64_t b = blockIdx.x / chunks;
+    const int first = (blockIdx.x - static_cast<int>(b) * chunks) * kFinalizeGroups;
+    collect_groups<kThreads>(partial, b, first, min(kFinalizeGroups, g.groups - first), g, eps,
+                             [&](int group, float2 v) { stats[b * g.groups + first + group] = v; });
+}
+
+// A thread's affine terms: y = (x - mean) * scale + shift per channel; weight and bias are loaded before the statistics are
+// there.  stat(group) gives {mean, inverse}.
+template <int V>
+__device__ __forceinline__ void load_affine(int c0, const void* weight, int w_dt, const void* bias, int b_dt, float (&scale)[V], float (&shift)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        scale[e] = weight ? load1(weight, w_dt, c0 + e) : 1.0f;
+        shift[e] = bias ? load1(bias, b_dt, c0 + e) : 0.0f;
     }
-    for (int offset = 16; offset > 0; offset >>= 1) {
-        s += __shfl_xor_sync(0xffffffffu, s, offset);
-        q += __shfl_xor_sync(0xffffffffu, q, offset);
-    }
-    if (lane == 0) {
-        const double n = static_cast<double>(g.spatial) * g.per, mean = s / n;
-        double var = q / n - mean * mean;
-        if (var < 0.0) var = 0.0;
-        stats[unit * 2] = static_cast<float>(mean);
-        stats[unit * 2 + 1] = static_cast<float>(1.0 / sqrt(var + static_cast<double>(eps)));
+}
+template <int V, typename Stat>
+__device__ __forceinline__ void apply_stats(const GclGeom& g, int c0, Stat stat, float (&mean)[V], float (&scale)[V]) {
+    int group = c0 / g.per, within = c0 - group * g.per;
+    float2 v = stat(group);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        mean[e] = v.x;
+        scale[e] *= v.y;
+        if (++within == g.per && e + 1 < V) { within = 0; v = stat(++group); }
     }
 }
 
+// stats: finished, or nullptr: every CTA adds the CTAs' sums of its batch entry (groups <= kInlineGroups)
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads, 4) gcl_apply_kernel(const T* x, const void* weight, int w_dt, const void* bias, int b_dt,
-                                                               T* out, const float* __restrict__ stats, GclGeom g, int ctas, int kind) {
+__global__ void __launch_bounds__(kThreads, 2) gcl_apply_kernel(const T* x, const void* weight, int w_dt, const void* bias, int b_dt, T* out,
+                                                               const double* __restrict__ partial, const float2* __restrict__ stats, GclGeom g, float eps,
+                                                               int ctas, int kind) {
+    __shared__ float2 own[kInlineGroups];
     pdl_wait();
     const int slabs = (g.vectors + g.slab - 1) / g.slab;
     const int unit = blockIdx.x / ctas, cta = ctas - 1 - (blockIdx.x - unit * ctas);
     const int b = unit / slabs, slab0 = (unit - b * slabs) * g.slab;
     const int lane_vector = threadIdx.x % g.slab, lane_row = threadIdx.x / g.slab;
-    if (lane_row >= g.rpp || slab0 + lane_vector >= g.vectors) return;
+    const bool live = lane_row < g.rpp && slab0 + lane_vector < g.vectors;
     const int c0 = (slab0 + lane_vector) * V;
     float mean[V], scale[V], shift[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-        const int64_t at = (static_cast<int64_t>(b) * g.groups + (c0 + e) / g.per) * 2;
-        mean[e] = stats[at];
-        scale[e] = stats[at + 1] * (weight ? load1(weight, w_dt, c0 + e) : 1.0f);
-        shift[e] = bias ? load1(bias, b_dt, c0 + e) : 0.0f;
-    }
+    if (live) load_affine<V>(c0, weight, w_dt, bias, b_dt, scale, shift);
+    if (stats == nullptr) collect_groups<kThreads>(partial, b, 0, g.groups, g, eps, [&](int group, float2 v) { own[group] = v; });
+    if (!live) return;
+    apply_stats<V>(g, c0, [&](int group) { return stats ? stats[static_cast<int64_t>(b) * g.groups + group] : own[group]; }, mean, scale);
     constexpr int U = 4;
     const int64_t step = static_cast<int64_t>(ctas) * g.rpp, p_step = step * g.channels;
     // rows of this thread are cta * rpp + lane_row + i * step, visited from the last one down
@@ -239,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 4) gcl_apply_kernel(const T* x, cons
         Vec<T, V> v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (row - u * step >= 0) v[u] = load_vec<T, V>(x + at - u * p_step);
+            if (row - u * step >= 0) v[u] = load_vec<true, T, V>(x + at - u * p_step);
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (row - u * step >= 0) {
@@ -251,10 +345,83 @@ __global__ void __launch_bounds__(kThreads, 4) gcl_apply_kernel(const T* x, cons
     }
 }
 
-int vector_width(int dtype, int64_t channels, const void* x, const void* out) {
+// One cluster per (batch entry, slab of whole groups): R rows of a thread stay in registers between the statistics and the
+// result.  Row i of a thread is (i * cluster + rank) * rpp + lane_row.
+template <typename T, int V, bool WHOLE, int ACT, int R>
+__global__ void __launch_bounds__(kClusterThreads) gcl_cluster_kernel(const T* x, const void* weight, int w_dt, const void* bias, int b_dt, T* out, GclGeom g,
+                                                              float eps, int kind) {
+    using Acc = Sums<T, V, WHOLE>;
+    __shared__ double sums[2][kClusterThreads * Acc::D];
+    __shared__ double mine[kClusterGroups][2];
+    __shared__ float2 own[kClusterGroups];
+    const int unit = blockIdx.x / g.cluster, rank = blockIdx.x - unit * g.cluster;
+    const int slabs = (g.vectors + g.slab - 1) / g.slab, b = unit / slabs, slab0 = (unit - b * slabs) * g.slab;
+    const int slab = min(g.slab, g.vectors - slab0);
+    const int lane_vector = threadIdx.x % g.slab, lane_row = threadIdx.x / g.slab;
+    const bool live = lane_row < g.rpp && lane_vector < slab;
+    const int row0 = rank * g.rpp + lane_row, step = g.cluster * g.rpp, spatial = static_cast<int>(g.spatial);
+    const int64_t at0 = (static_cast<int64_t>(b) * g.spatial + row0) * g.channels + (slab0 + lane_vector) * V;
+    const int64_t p_step = static_cast<int64_t>(step) * g.channels;
+    pdl_wait();
+    Vec<T, V> v[R];
+    Acc acc;
+    acc.clear();
+    const int c0 = (slab0 + lane_vector) * V;
+    float scale[V], shift[V];
+    if (live) load_affine<V>(c0, weight, w_dt, bias, b_dt, scale, shift);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+        if (live && row0 + i * step < spatial) v[i] = load_vec<true, T, V>(x + at0 + i * p_step);
+    if (live && row0 < spatial) {
+        acc.begin(v[0]);
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (row0 + i * step < spatial) { acc.add(v[i]); ++n; }
+        acc.rebuild(n);
+    }
+#pragma unroll
+    for (int e = 0; e < Acc::D; ++e) {
+        sums[0][threadIdx.x * Acc::D + e] = acc.S[e];
+        sums[1][threadIdx.x * Acc::D + e] = acc.Q[e];
+    }
+    __syncthreads();
+    add_groups<kClusterThreads, Acc::D, V>(sums, g, slab0, slab, [&](int group, double s, double q) { mine[group][0] = s; mine[group][1] = q; });
+    if (g.cluster > 1) cluster_sync(); else __syncthreads();
+    const int groups = slab * V / g.per;
+    for (int group = threadIdx.x; group < groups; group += kClusterThreads) {
+        double s = 0.0, q = 0.0;
+        for (int r = 0; r < g.cluster; ++r) {
+            s += g.cluster > 1 ? load_cluster(&mine[group][0], r) : mine[group][0];
+            q += g.cluster > 1 ? load_cluster(&mine[group][1], r) : mine[group][1];
+        }
+        own[group] = moments_to_stats(s, q, g.share, eps);
+    }
+    __syncthreads();
+    if (live) {
+        const int first = slab0 * V / g.per;
+        float mean[V];
+        apply_stats<V>(g, c0, [&](int group) { return own[group - first]; }, mean, scale);
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (row0 + i * step < spatial) {
+                float y[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) y[e] = activate<ACT>(fmaf(v[i].get(e) - mean[e], scale[e], shift[e]), kind);
+                store_vec<V>(out + at0 + i * p_step, y);
+            }
+    }
+    if (g.cluster > 1) cluster_sync();   // no CTA's memory goes while another reads it
+}
+
+// Elements of a vector: the most that divide the row and the tensors' alignment, up to 16 bytes.  Eight bf16 channels only where
+// they lie in one group: eight pairs of double sums a thread are more than the registers take.
+int vector_width(int dtype, int64_t channels, int groups, const void* x, const void* out) {
     const int element = static_cast<int>(dtype_bytes(dtype));
     for (int v = 16 / element; v > 1; v /= 2)
-        if (channels % v == 0 && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) % (v * element)) == 0) return v;
+        if (channels % v == 0 && (v < 8 || channels / groups % v == 0) &&
+            ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) % (v * element)) == 0)
+            return v;
     return 1;
 }
 
@@ -265,50 +432,132 @@ int make_geom(GclGeom& g, int64_t batch, int64_t spatial, int64_t channels, int 
                 "group_norm_channels_last: group norm launch extent exceeds CUDA grid capacity");
     g.batch = batch; g.spatial = spatial;
     g.channels = static_cast<int>(channels); g.groups = groups; g.per = static_cast<int>(channels / groups);
+    g.share = 1.0 / (static_cast<double>(spatial) * g.per);
     return VRB_OK;
-}
-// CTAs of the statistics pass per batch entry: kSplitsPerSm per SM over the whole batch, none without a row.  Depends on
-// V only through rpp, so the workspace is sized with the most a layout can ask for.
-int splits_for(const GclGeom& g, int rpp) {
-    int64_t want = (static_cast<int64_t>(sm_count()) * kSplitsPerSm + g.batch - 1) / g.batch;
-    const int64_t most = (g.spatial + rpp - 1) / rpp;
-    if (want > most) want = most;
-    return static_cast<int>(want < 1 ? 1 : want);
 }
 void set_width(GclGeom& g, int v) {
     g.vectors = g.channels / v;
     g.slab = g.vectors < kThreads ? g.vectors : kThreads;
     g.rpp = kThreads / g.slab;
     if (g.rpp > g.spatial) g.rpp = static_cast<int>(g.spatial);
-    g.splits = splits_for(g, g.rpp);
 }
+// CTAs of the statistics pass per batch entry: one per SM over the whole batch, no more than passes over the rows
+void set_splits(GclGeom& g) {
+    const int64_t want = (sm_count() + g.batch - 1) / g.batch, most = (g.spatial + g.rpp - 1) / g.rpp;
+    g.splits = static_cast<int>(want < most ? want : most);
+}
+// The slab and cluster of gcl_cluster, or false: the slab is the least run of whole groups and whole vectors of 64 bytes or
+// more (a row's piece of a slab should fill memory sectors), its rows have to fit `rows` registers of up to eight CTAs.  Above
+// kClusterBytes the second read of x comes out of L2 as fast as the clusters hand out work: measured at 512 channels bf16,
+// 256 rows 4.3 us against 9.2, 4096 rows 6.4 against 11.3, 8192 rows 10.3 against 12.2, 16384 rows 20 against 16.
+constexpr int64_t kClusterBytes = int64_t{8} << 20;
+bool set_cluster(GclGeom& g, int v, int element, int rows) {
+    if (g.batch * g.spatial * g.channels * element > kClusterBytes) return false;
+    int groups = 1;
+    while (groups < g.groups && (groups * g.per % v != 0 || groups * g.per * element < 64 || g.groups % groups != 0)) ++groups;
+    const int64_t slab = static_cast<int64_t>(groups) * g.per;
+    if (slab % v != 0 || slab / v > kClusterThreads || groups > kClusterGroups) return false;
+    g.vectors = g.channels / v;
+    g.slab = static_cast<int>(slab / v);
+    g.rpp = kClusterThreads / g.slab;
+    if (g.rpp > g.spatial) g.rpp = static_cast<int>(g.spatial);
+    const int64_t passes = (g.spatial + g.rpp - 1) / g.rpp;
+    g.cluster = static_cast<int>(passes < 8 ? passes : 8);
+    return passes <= static_cast<int64_t>(g.cluster) * rows;
+}
+constexpr int kMostRows = 16;      // rows of a thread that gcl_cluster keeps
 
 size_t up256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
-size_t partial_bytes(const GclGeom& g) { return up256(static_cast<size_t>(g.batch) * splits_for(g, 1) * g.groups * 2 * sizeof(double)); }
-size_t workspace_size(const GclGeom& g) { return partial_bytes(g) + up256(static_cast<size_t>(g.batch) * g.groups * 2 * sizeof(float)); }
+// the most any vector width asks for
+size_t partial_bytes(const GclGeom& g) {
+    const int64_t ctas = sm_count() + g.batch;
+    return up256(static_cast<size_t>(ctas) * g.groups * 2 * sizeof(double));
+}
+size_t workspace_size(const GclGeom& g) {
+    return partial_bytes(g) + (g.groups > kInlineGroups ? up256(static_cast<size_t>(g.batch) * g.groups * sizeof(float2)) : 0);
+}
+
+template <typename... KArgs, typename... Args>
+void launch_clusters(void (*kernel)(KArgs...), unsigned ctas, int cluster, cudaStream_t stream, Args&&... args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(ctas);
+    config.blockDim = dim3(kClusterThreads);
+    config.stream = stream;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeClusterDimension;
+    attributes[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+    attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[1].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attributes;
+    config.numAttrs = g_launch_overlap.load(std::memory_order_relaxed) != 0 ? 2 : 1;
+    cudaLaunchKernelEx(&config, kernel, static_cast<KArgs>(args)...);   // an error stays for after_launch()
+}
+
+struct GclCall {
+    const void *x, *weight, *bias;
+    void* out;
+    int w_dt, b_dt, activation;
+    float eps;
+};
+
+template <typename T, int V, bool WHOLE, int ACT>
+int run_cluster(const GclCall& c, const GclGeom& g, cudaStream_t s) {
+    const int64_t units = g.batch * ((g.vectors + g.slab - 1) / g.slab), passes = (g.spatial + g.rpp - 1) / g.rpp;
+    const int rows = static_cast<int>((passes + g.cluster - 1) / g.cluster);
+#define VRB_GCL_CLUSTER(R) launch_clusters(gcl_cluster_kernel<T, V, WHOLE, ACT, R>, static_cast<unsigned>(units * g.cluster), g.cluster, s, static_cast<const T*>(c.x), \
+                                           c.weight, c.w_dt, c.bias, c.b_dt, static_cast<T*>(c.out), g, c.eps, c.activation)
+    if (rows <= 4) VRB_GCL_CLUSTER(4);
+    else VRB_GCL_CLUSTER(kMostRows);
+#undef VRB_GCL_CLUSTER
+    return after_launch("group_norm_channels_last");
+}
+template <typename T, int V, bool WHOLE>
+int run_cluster(const GclCall& c, const GclGeom& g, cudaStream_t s) {
+    if (c.activation == VRB_NO_ACTIVATION) return run_cluster<T, V, WHOLE, 0>(c, g, s);
+    if (c.activation == VRB_SILU) return run_cluster<T, V, WHOLE, 1>(c, g, s);
+    if (c.activation == VRB_GELU_TANH) return run_cluster<T, V, WHOLE, 2>(c, g, s);
+    return run_cluster<T, V, WHOLE, 3>(c, g, s);
+}
 
 template <typename T, int V>
-int run_two_pass(const T* x, const void* weight, int w_dt, const void* bias, int b_dt, T* out, GclGeom g, float eps, int activation,
-                 char* workspace, cudaStream_t s) {
+int run_passes(const GclCall& c, GclGeom g, char* workspace, cudaStream_t s) {
     set_width(g, V);
+    set_splits(g);
     double* partial = reinterpret_cast<double*>(workspace);
-    float* stats = reinterpret_cast<float*>(workspace + partial_bytes(g));
-    launch_overlapped(gcl_partial_kernel<T, V>, dim3(static_cast<unsigned>(g.batch * g.splits)), dim3(kThreads), 0, s, x, partial, g);
+    float2* stats = g.groups > kInlineGroups ? reinterpret_cast<float2*>(workspace + partial_bytes(g)) : nullptr;
+    const dim3 ctas_stats(static_cast<unsigned>(g.batch * g.splits));
+    const T* x = static_cast<const T*>(c.x);
+    if (g.per % V == 0) launch_overlapped(gcl_partial_kernel<T, V, true>, ctas_stats, dim3(kThreads), 0, s, x, partial, g);
+    else if constexpr (V > 1 && V < 8) launch_overlapped(gcl_partial_kernel<T, V, false>, ctas_stats, dim3(kThreads), 0, s, x, partial, g);
     if (int rc = after_launch("group_norm_channels_last statistics")) return rc;
-    launch_overlapped(gcl_finalize_kernel, dim3(static_cast<unsigned>((g.batch * g.groups * 32 + 127) / 128)), dim3(128), 0, s, partial, stats, g, eps);
-    if (int rc = after_launch("group_norm_channels_last finalize")) return rc;
+    if (stats) {
+        launch_overlapped(gcl_finalize_kernel, dim3(static_cast<unsigned>(g.batch * ((g.groups + kFinalizeGroups - 1) / kFinalizeGroups))), dim3(kThreads), 0, s, partial,
+                          stats, g, c.eps);
+        if (int rc = after_launch("group_norm_channels_last finalize")) return rc;
+    }
     const int64_t slabs = (g.vectors + g.slab - 1) / g.slab, units = g.batch * slabs;
-    int64_t ctas = (static_cast<int64_t>(sm_count()) * 8 + units - 1) / units;
+    int64_t ctas = (static_cast<int64_t>(sm_count()) * 2 + units - 1) / units;
     const int64_t most = (g.spatial + g.rpp - 1) / g.rpp;
     if (ctas > most) ctas = most;
     const dim3 grid(static_cast<unsigned>(units * ctas));
-#define VRB_GCL_APPLY(ACT) launch_overlapped(gcl_apply_kernel<T, V, ACT>, grid, dim3(kThreads), 0, s, x, weight, w_dt, bias, b_dt, out, stats, g, static_cast<int>(ctas), activation)
-    if (activation == VRB_NO_ACTIVATION) VRB_GCL_APPLY(0);
-    else if (activation == VRB_SILU) VRB_GCL_APPLY(1);
-    else if (activation == VRB_GELU_TANH) VRB_GCL_APPLY(2);
+#define VRB_GCL_APPLY(ACT) launch_overlapped(gcl_apply_kernel<T, V, ACT>, grid, dim3(kThreads), 0, s, static_cast<const T*>(c.x), c.weight, c.w_dt, c.bias, c.b_dt, \
+                                             static_cast<T*>(c.out), partial, stats, g, c.eps, static_cast<int>(ctas), c.activation)
+    if (c.activation == VRB_NO_ACTIVATION) VRB_GCL_APPLY(0);
+    else if (c.activation == VRB_SILU) VRB_GCL_APPLY(1);
+    else if (c.activation == VRB_GELU_TANH) VRB_GCL_APPLY(2);
     else VRB_GCL_APPLY(3);
 #undef VRB_GCL_APPLY
     return after_launch("group_norm_channels_last apply");
+}
+
+template <typename T, int V>
+int run_width(const GclCall& c, GclGeom g, bool cluster, char* workspace, cudaStream_t s) {
+    if (!cluster) return run_passes<T, V>(c, g, workspace, s);
+    set_cluster(g, V, sizeof(T), kMostRows);
+    if constexpr (V > 1 && V < 8)
+        if (g.per % V != 0) return run_cluster<T, V, false>(c, g, s);
+    return run_cluster<T, V, true>(c, g, s);
 }
 
 }  // namespace
@@ -319,7 +568,14 @@ using namespace vrb;
 extern "C" size_t vrb_group_norm_channels_last_workspace_bytes(int dtype, int64_t batch, int64_t spatial, int64_t channels, int groups) {
     GclGeom g;
     if (!is_float_dtype(dtype) || make_geom(g, batch, spatial, channels, groups)) return 0;
-    return workspace_size(g);
+    // none where the cluster kernel takes the shape at every alignment a tensor can have
+    const int element = static_cast<int>(dtype_bytes(dtype));
+    bool cluster = true;
+    for (int v = 16 / element; v >= 1 && cluster; v /= 2) {
+        GclGeom h = g;
+        if (channels % v == 0 && (v < 8 || h.per % v == 0)) cluster = set_cluster(h, v, element, kMostRows);
+    }
+    return cluster ? 0 : workspace_size(g);
 }
 
 extern "C" int vrb_group_norm_channels_last(const void* x, int dtype, const void* weight, int weight_dtype,
@@ -334,21 +590,22 @@ extern "C" int vrb_group_norm_channels_last(const void* x, int dtype, const void
                 "group_norm_channels_last: unknown activation %d", activation);
     GclGeom g;
     if (int rc = make_geom(g, batch, spatial, channels, groups)) return rc;
-    const size_t need = workspace_size(g);
-    VRB_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, VRB_ERR_WORKSPACE,
+    const int v = vector_width(dtype, channels, groups, x, out);
+    GclGeom h = g;
+    const bool cluster = set_cluster(h, v, static_cast<int>(dtype_bytes(dtype)), kMostRows);
+    const size_t need = cluster ? 0 : workspace_size(g);
+    VRB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0), VRB_ERR_WORKSPACE,
                 "group_norm_channels_last: workspace needs %zu bytes, 256-byte aligned", need);
     char* ws = static_cast<char*>(workspace);
     cudaStream_t s = as_stream(stream);
-#define VRB_GCL_RUN(T, V) run_two_pass<T, V>(static_cast<const T*>(x), weight, weight_dtype, bias, bias_dtype, static_cast<T*>(out), g, eps, activation, ws, s)
-    const int v = vector_width(dtype, channels, x, out);
+    const GclCall c{x, weight, bias, out, weight_dtype, bias_dtype, activation, eps};
     if (dtype == VRB_BF16) {
-        if (v == 8) return VRB_GCL_RUN(uint16_t, 8);
-        if (v == 4) return VRB_GCL_RUN(uint16_t, 4);
-        if (v == 2) return VRB_GCL_RUN(uint16_t, 2);
-        return VRB_GCL_RUN(uint16_t, 1);
+        if (v == 8) return run_width<uint16_t, 8>(c, g, cluster, ws, s);
+        if (v == 4) return run_width<uint16_t, 4>(c, g, cluster, ws, s);
+        if (v == 2) return run_width<uint16_t, 2>(c, g, cluster, ws, s);
+        return run_width<uint16_t, 1>(c, g, cluster, ws, s);
     }
-    if (v == 4) return VRB_GCL_RUN(float, 4);
-    if (v == 2) return VRB_GCL_RUN(float, 2);
-    return VRB_GCL_RUN(float, 1);
-#undef VRB_GCL_RUN
+    if (v == 4) return run_width<float, 4>(c, g, cluster, ws, s);
+    if (v == 2) return run_width<float, 2>(c, g, cluster, ws, s);
+    return run_width<float, 1>(c, g, cluster, ws, s);
 }
