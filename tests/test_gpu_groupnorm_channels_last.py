@@ -47,6 +47,9 @@ SHAPES = [
     ((1, 1, 1), 1), ((2, 1, 64), 32), ((1, 2, 8), 8), ((3, 7, 3), 3), ((2, 33, 6), 2), ((1, 1, 320), 32), ((1, 5, 24), 4),
     ((1, 256, 512), 32), ((2, 16, 16, 128), 32), ((3, 1035, 320), 32), ((1, 3, 20, 30, 96), 8), ((2, 500, 36), 12), ((1, 700, 7), 1),
     ((1, 4000, 50), 5), ((5, 64, 64), 1), ((2, 9, 2560), 32), ((1, 40, 4096), 2), ((1, 33, 4112), 16), ((1, 17, 2050), 2),
+    # rows that are no whole vectors, folded, with and without a rest
+    ((1, 200003, 1), 1), ((1, 60001, 3), 1), ((1, 60001, 3), 3), ((1, 50001, 10), 1), ((1, 50000, 10), 5), ((1, 33333, 30), 10),
+    ((2, 40000, 5), 1), ((2, 40001, 5), 5), ((3, 20001, 12), 4), ((1, 9001, 100), 25), ((1, 5003, 402), 6), ((1, 3001, 2001), 3),
     ((1, 60000, 64), 8), ((1, 30000, 100), 4), ((4, 3000, 40), 8), ((1, 24960, 128), 32), ((300, 5, 16), 4),
 ]
 

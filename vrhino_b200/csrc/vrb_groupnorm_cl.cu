@@ -25,9 +25,13 @@ constexpr int kRun = 32;           // rows of a thread between two rebuilds in d
 constexpr int kClusterGroups = 128;// groups of a cluster's slab, at most
 constexpr int kInlineGroups = 64;  // groups up to which gcl_apply adds the CTAs' sums itself
 
+// Rows whose byte count is no multiple of a vector's are folded: `fold` of them make a row of whole vectors, and what is left of
+// the last such row (`tail` elements) is handled element by element.
 struct GclGeom {
-    int64_t batch, spatial;
-    int channels, groups, per;     // per = channels / groups
+    int64_t batch, spatial;        // spatial: folded rows
+    int64_t entry;                 // elements of a batch entry
+    int channels, groups, per;     // channels: elements of a folded row; per: channels of a group
+    int fold, row, tail;           // row: elements of an unfolded row
     int vectors;                   // channels / V
     int slab;                      // vectors a CTA covers at a time (<= kThreads)
     int rpp;                       // rows a CTA covers at a time
@@ -36,11 +40,6 @@ struct GclGeom {
     double share;                  // 1 / elements of a group
 };
 
-__device__ __forceinline__ unsigned cluster_rank() {
-    unsigned r;
-    asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
-    return r;
-}
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory"); }
 // the double at `local` in the shared memory of the cluster's CTA `rank`
 __device__ __forceinline__ double load_cluster(const double* local, unsigned rank) {
@@ -134,6 +133,11 @@ struct Sums {
             s2[0] = fmaf(d, d, s2[0]);
         }
     }
+    __device__ __forceinline__ void single(int e, float v) {
+        const double d = v;
+        S[WHOLE ? 0 : e] += d;
+        Q[WHOLE ? 0 : e] += d * d;
+    }
     __device__ __forceinline__ void rebuild(int n) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
@@ -150,6 +154,24 @@ template <int THREADS, int D, int V, typename Take>
 __device__ __forceinline__ void add_groups(double (&sums)[2][THREADS * D], const GclGeom& g, int slab0, int slab, Take take) {
     const int lane = threadIdx.x & 31, c_begin = slab0 * V, c_end = c_begin + slab * V, first = c_begin / g.per;
     constexpr int E = V / D;   // channels of an entry
+    if (g.fold > 1) {          // one slab; a group's channels come `fold` times
+        const int width = g.per * (g.groups == 1 ? g.fold : 1) / E, times = g.groups == 1 ? 1 : g.fold;
+        for (int group = threadIdx.x >> 5; group < g.groups; group += THREADS / 32) {
+            double s = 0.0, q = 0.0;
+            for (int i = lane; i < g.rpp * times * width; i += 32) {
+                const int r = i / (times * width), j = (i - r * times * width) / width, at = i - (r * times + j) * width;
+                const int k = r * g.slab * D + (j * g.row + group * g.per) / E + at;
+                s += sums[0][k];
+                q += sums[1][k];
+            }
+            for (int offset = 16; offset > 0; offset >>= 1) {
+                s += __shfl_xor_sync(0xffffffffu, s, offset);
+                q += __shfl_xor_sync(0xffffffffu, q, offset);
+            }
+            if (lane == 0) take(group, s, q);
+        }
+        return;
+    }
     for (int group = first + (threadIdx.x >> 5); group * g.per < c_end; group += THREADS / 32) {
         const int from = (max(group * g.per, c_begin) - c_begin) / E, width = (min((group + 1) * g.per, c_end) - c_begin) / E - from;
         double s = 0.0, q = 0.0;
@@ -184,6 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1) gcl_partial_kernel(const T* x, do
     using Acc = Sums<T, V, WHOLE>;
     __shared__ double sums[2][kThreads * Acc::D];
     pdl_wait();
+    pdl_launch_dependents();   // gcl_apply reads x, weight and bias ahead of its own wait: all of them are there from here on
     const int b = blockIdx.x / g.splits, split = blockIdx.x - b * g.splits;
     const int lane_vector = threadIdx.x % g.slab, lane_row = threadIdx.x / g.slab;
     double* out = partial + static_cast<int64_t>(blockIdx.x) * g.groups * 2;
@@ -195,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1) gcl_partial_kernel(const T* x, do
             constexpr int U = WHOLE && sizeof(T) * V == 16 ? 8 : 4;
             const int64_t step = static_cast<int64_t>(g.splits) * g.rpp, p_step = step * g.channels;
             const int64_t row = static_cast<int64_t>(split) * g.rpp + lane_row;
-            const T* p = x + (static_cast<int64_t>(b) * g.spatial + row) * g.channels + (slab0 + lane_vector) * V;
+            const T* p = x + b * g.entry + row * g.channels + (slab0 + lane_vector) * V;
             int64_t left = row < g.spatial ? (g.spatial - 1 - row) / step + 1 : 0;   // rows of this thread from p on
             // U rows at a time, the next U on their way while these are added
             Vec<T, V> now[U], next[U];
@@ -224,6 +247,12 @@ __global__ void __launch_bounds__(kThreads, 1) gcl_partial_kernel(const T* x, do
                 }
 #pragma unroll
                 for (int u = 0; u < U; ++u) now[u] = next[u];
+            }
+            if (g.tail > 0 && row <= g.spatial && (g.spatial - row) % step == 0) {
+                const T* rest = x + b * g.entry + g.spatial * g.channels;
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (lane_vector * V + e < g.tail) acc.single(e, load1(rest, sizeof(T) == 2 ? VRB_BF16 : VRB_F32, lane_vector * V + e));
             }
         }
         if (slab0) __syncthreads();
@@ -285,13 +314,22 @@ __global__ void __launch_bounds__(kThreads) gcl_finalize_kernel(const double* __
 // A thread's affine terms: y = (x - mean) * scale + shift per channel; weight and bias are loaded before the statistics are
 // there.  stat(group) gives {mean, inverse}.
 template <int V>
-__device__ __forceinline__ void load_affine(int c0, const void* weight, int w_dt, const void* bias, int b_dt, float (&scale)[V], float (&shift)[V]) {
+__device__ __forceinline__ void load_channels(const void* p, int dt, int c0, int channels, float fill, float (&v)[V]) {
+    if (p == nullptr) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-        scale[e] = weight ? load1(weight, w_dt, c0 + e) : 1.0f;
-        shift[e] = bias ? load1(bias, b_dt, c0 + e) : 0.0f;
+        for (int e = 0; e < V; ++e) v[e] = fill;
+        return;
+    }
+    int c = c0;
+    if (dt == VRB_F32) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) { v[e] = static_cast<const float*>(p)[c]; if (++c == channels) c = 0; }
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) { v[e] = bf16_bits_to_float(static_cast<const uint16_t*>(p)[c]); if (++c == channels) c = 0; }
     }
 }
+// c0: the first channel, modulo the unfolded row
 template <int V, typename Stat>
 __device__ __forceinline__ void apply_stats(const GclGeom& g, int c0, Stat stat, float (&mean)[V], float (&scale)[V]) {
     int group = c0 / g.per, within = c0 - group * g.per;
@@ -300,7 +338,11 @@ __device__ __forceinline__ void apply_stats(const GclGeom& g, int c0, Stat stat,
     for (int e = 0; e < V; ++e) {
         mean[e] = v.x;
         scale[e] *= v.y;
-        if (++within == g.per && e + 1 < V) { within = 0; v = stat(++group); }
+        if (++within == g.per && e + 1 < V) {
+            within = 0;
+            if (++group == g.groups) group = 0;
+            v = stat(group);
+        }
     }
 }
 
@@ -310,30 +352,33 @@ __global__ void __launch_bounds__(kThreads, 2) gcl_apply_kernel(const T* x, cons
                                                                const double* __restrict__ partial, const float2* __restrict__ stats, GclGeom g, float eps,
                                                                int ctas, int kind) {
     __shared__ float2 own[kInlineGroups];
-    pdl_wait();
     const int slabs = (g.vectors + g.slab - 1) / g.slab;
     const int unit = blockIdx.x / ctas, cta = ctas - 1 - (blockIdx.x - unit * ctas);
     const int b = unit / slabs, slab0 = (unit - b * slabs) * g.slab;
     const int lane_vector = threadIdx.x % g.slab, lane_row = threadIdx.x / g.slab;
     const bool live = lane_row < g.rpp && slab0 + lane_vector < g.vectors;
-    const int c0 = (slab0 + lane_vector) * V;
-    float mean[V], scale[V], shift[V];
-    if (live) load_affine<V>(c0, weight, w_dt, bias, b_dt, scale, shift);
-    if (stats == nullptr) collect_groups<kThreads>(partial, b, 0, g.groups, g, eps, [&](int group, float2 v) { own[group] = v; });
-    if (!live) return;
-    apply_stats<V>(g, c0, [&](int group) { return stats ? stats[static_cast<int64_t>(b) * g.groups + group] : own[group]; }, mean, scale);
+    const int c0 = (slab0 + lane_vector) * V, channel = g.fold > 1 ? c0 % g.row : c0;
     constexpr int U = 4;
     const int64_t step = static_cast<int64_t>(ctas) * g.rpp, p_step = step * g.channels;
-    // rows of this thread are cta * rpp + lane_row + i * step, visited from the last one down
-    int64_t row = static_cast<int64_t>(cta) * g.rpp + lane_row;
-    if (row >= g.spatial) return;
-    row += (g.spatial - 1 - row) / step * step;
-    int64_t at = (static_cast<int64_t>(b) * g.spatial + row) * g.channels + c0;
-    for (; row >= 0; row -= U * step, at -= U * p_step) {
-        Vec<T, V> v[U];
+    // rows of this thread are cta * rpp + lane_row + i * step, visited from the last one down; the first U of them are on their
+    // way before the statistics are waited for (gcl_partial began after everything before it had ended)
+    const int64_t row0 = static_cast<int64_t>(cta) * g.rpp + lane_row;
+    int64_t row = row0 < g.spatial ? row0 + (g.spatial - 1 - row0) / step * step : -1;
+    int64_t at = b * g.entry + row * g.channels + c0;
+    Vec<T, V> v[U];
+    float mean[V], scale[V], shift[V];
+    if (live) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (row - u * step >= 0) v[u] = load_vec<true, T, V>(x + at - u * p_step);
+        load_channels<V>(weight, w_dt, channel, g.row, 1.0f, scale);
+        load_channels<V>(bias, b_dt, channel, g.row, 0.0f, shift);
+    }
+    pdl_wait();
+    if (stats == nullptr) collect_groups<kThreads>(partial, b, 0, g.groups, g, eps, [&](int group, float2 v) { own[group] = v; });
+    if (!live) return;
+    apply_stats<V>(g, channel, [&](int group) { return stats ? stats[static_cast<int64_t>(b) * g.groups + group] : own[group]; }, mean, scale);
+    while (row >= 0) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (row - u * step >= 0) {
@@ -342,12 +387,25 @@ __global__ void __launch_bounds__(kThreads, 2) gcl_apply_kernel(const T* x, cons
                 for (int e = 0; e < V; ++e) y[e] = activate<ACT>(fmaf(v[u].get(e) - mean[e], scale[e], shift[e]), kind);
                 store_vec<V>(out + at - u * p_step, y);
             }
+        row -= U * step;
+        at -= U * p_step;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (row - u * step >= 0) v[u] = load_vec<true, T, V>(x + at - u * p_step);
+    }
+    if (g.tail > 0 && row0 <= g.spatial && (g.spatial - row0) % step == 0) {
+        constexpr int dt = sizeof(T) == 2 ? VRB_BF16 : VRB_F32;
+        const int64_t rest = b * g.entry + g.spatial * g.channels + c0;
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (c0 + e < g.tail) store1(out, dt, rest + e, activate<ACT>(fmaf(load1(x, dt, rest + e) - mean[e], scale[e], shift[e]), kind));
     }
 }
 
-// One cluster per (batch entry, slab of whole groups): R rows of a thread stay in registers between the statistics and the
-// result.  Row i of a thread is (i * cluster + rank) * rpp + lane_row.
-template <typename T, int V, bool WHOLE, int ACT, int R>
+// One cluster per (batch entry, slab of whole groups): up to kMostRows rows of a thread stay in registers between the statistics
+// and the result.  Row i of a thread is (i * cluster + rank) * rpp + lane_row.
+constexpr int kMostRows = 4;
+template <typename T, int V, bool WHOLE, int ACT>
 __global__ void __launch_bounds__(kClusterThreads) gcl_cluster_kernel(const T* x, const void* weight, int w_dt, const void* bias, int b_dt, T* out, GclGeom g,
                                                               float eps, int kind) {
     using Acc = Sums<T, V, WHOLE>;
@@ -363,15 +421,19 @@ __global__ void __launch_bounds__(kClusterThreads) gcl_cluster_kernel(const T* x
     const int64_t at0 = (static_cast<int64_t>(b) * g.spatial + row0) * g.channels + (slab0 + lane_vector) * V;
     const int64_t p_step = static_cast<int64_t>(step) * g.channels;
     pdl_wait();
+    constexpr int R = kMostRows;
     Vec<T, V> v[R];
     Acc acc;
     acc.clear();
     const int c0 = (slab0 + lane_vector) * V;
-    float scale[V], shift[V];
-    if (live) load_affine<V>(c0, weight, w_dt, bias, b_dt, scale, shift);
 #pragma unroll
     for (int i = 0; i < R; ++i)
         if (live && row0 + i * step < spatial) v[i] = load_vec<true, T, V>(x + at0 + i * p_step);
+    float scale[V], shift[V];
+    if (live) {
+        load_channels<V>(weight, w_dt, c0, g.row, 1.0f, scale);
+        load_channels<V>(bias, b_dt, c0, g.row, 0.0f, shift);
+    }
     if (live && row0 < spatial) {
         acc.begin(v[0]);
         int n = 0;
@@ -414,45 +476,57 @@ __global__ void __launch_bounds__(kClusterThreads) gcl_cluster_kernel(const T* x
     if (g.cluster > 1) cluster_sync();   // no CTA's memory goes while another reads it
 }
 
-// Elements of a vector: the most that divide the row and the tensors' alignment, up to 16 bytes.  Eight bf16 channels only where
-// they lie in one group: eight pairs of double sums a thread are more than the registers take.
-int vector_width(int dtype, int64_t channels, int groups, const void* x, const void* out) {
+int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
+// Elements of a vector: the most, up to 16 bytes, for which every batch entry begins on a vector's boundary; rows that are no
+// multiple of it are folded where the folded row is not too long for a CTA.  Eight bf16 channels only where they lie in one
+// group: eight pairs of double sums a thread are more than the registers take.
+int vector_width(int dtype, int64_t batch, int64_t spatial, int64_t channels, int groups, bool fold, const void* x, const void* out) {
     const int element = static_cast<int>(dtype_bytes(dtype));
-    for (int v = 16 / element; v > 1; v /= 2)
-        if (channels % v == 0 && (v < 8 || channels / groups % v == 0) &&
-            ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) % (v * element)) == 0)
-            return v;
+    for (int v = 16 / element; v > 1; v /= 2) {
+        const int64_t folded = channels / gcd(static_cast<int>(channels), v);
+        if (channels % v != 0 && (!fold || folded > kThreads || spatial < v || (batch > 1 && spatial * channels % v != 0))) continue;
+        if (v == 8 && groups > 1 && channels / groups % 8 != 0) continue;
+        if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) % (v * element) == 0) return v;
+    }
     return 1;
 }
+// Whether the V channels of a vector always lie in one group
+bool one_group(const GclGeom& g, int v) { return g.groups == 1 || (g.row % v == 0 && g.per % v == 0); }
 
 int make_geom(GclGeom& g, int64_t batch, int64_t spatial, int64_t channels, int groups) {
     VRB_REQUIRE(batch > 0 && spatial > 0 && channels > 0 && groups > 0 && channels % groups == 0, VRB_ERR_INVALID,
                 "group_norm_channels_last: group norm shape/groups mismatch");
     VRB_REQUIRE(channels <= (int64_t{1} << 24) && batch <= (int64_t{1} << 20), VRB_ERR_INVALID,
                 "group_norm_channels_last: group norm launch extent exceeds CUDA grid capacity");
-    g.batch = batch; g.spatial = spatial;
-    g.channels = static_cast<int>(channels); g.groups = groups; g.per = static_cast<int>(channels / groups);
+    g.batch = batch; g.spatial = spatial; g.entry = spatial * channels;
+    g.channels = g.row = static_cast<int>(channels); g.fold = 1; g.tail = 0; g.groups = groups; g.per = static_cast<int>(channels / groups);
     g.share = 1.0 / (static_cast<double>(spatial) * g.per);
     return VRB_OK;
 }
+int64_t all_rows(const GclGeom& g) { return g.spatial + (g.tail > 0 ? 1 : 0); }
 void set_width(GclGeom& g, int v) {
+    if (g.row % v != 0) {
+        g.fold = v / gcd(g.row, v);
+        g.channels = g.row * g.fold;
+        g.spatial = g.entry / g.channels;
+        g.tail = static_cast<int>(g.entry - g.spatial * g.channels);
+    }
     g.vectors = g.channels / v;
     g.slab = g.vectors < kThreads ? g.vectors : kThreads;
     g.rpp = kThreads / g.slab;
-    if (g.rpp > g.spatial) g.rpp = static_cast<int>(g.spatial);
+    if (g.rpp > all_rows(g)) g.rpp = static_cast<int>(all_rows(g));
 }
 // CTAs of the statistics pass per batch entry: one per SM over the whole batch, no more than passes over the rows
 void set_splits(GclGeom& g) {
-    const int64_t want = (sm_count() + g.batch - 1) / g.batch, most = (g.spatial + g.rpp - 1) / g.rpp;
+    const int64_t want = (sm_count() + g.batch - 1) / g.batch, most = (all_rows(g) + g.rpp - 1) / g.rpp;
     g.splits = static_cast<int>(want < most ? want : most);
 }
 // The slab and cluster of gcl_cluster, or false: the slab is the least run of whole groups and whole vectors of 64 bytes or
-// more (a row's piece of a slab should fill memory sectors), its rows have to fit `rows` registers of up to eight CTAs.  Above
-// kClusterBytes the second read of x comes out of L2 as fast as the clusters hand out work: measured at 512 channels bf16,
-// 256 rows 4.3 us against 9.2, 4096 rows 6.4 against 11.3, 8192 rows 10.3 against 12.2, 16384 rows 20 against 16.
-constexpr int64_t kClusterBytes = int64_t{8} << 20;
-bool set_cluster(GclGeom& g, int v, int element, int rows) {
-    if (g.batch * g.spatial * g.channels * element > kClusterBytes) return false;
+// more (a row's piece of a slab should fill memory sectors), its rows have to fit kMostRows rows of a thread in up to eight
+// CTAs, and all clusters should be at work at once.  Measured against the passes (bf16 with SiLU, back to back): 64 rows of 512
+// channels 4.9 us against 8.8, 256 rows 5.7 against 9.2, 2048 rows 8.0 against 11.8; with 16 rows a thread the code of a
+// once-run kernel costs more than a second read of x (4096 rows 15.9 against 12.6).
+bool set_cluster(GclGeom& g, int v, int element) {
     int groups = 1;
     while (groups < g.groups && (groups * g.per % v != 0 || groups * g.per * element < 64 || g.groups % groups != 0)) ++groups;
     const int64_t slab = static_cast<int64_t>(groups) * g.per;
@@ -463,9 +537,8 @@ bool set_cluster(GclGeom& g, int v, int element, int rows) {
     if (g.rpp > g.spatial) g.rpp = static_cast<int>(g.spatial);
     const int64_t passes = (g.spatial + g.rpp - 1) / g.rpp;
     g.cluster = static_cast<int>(passes < 8 ? passes : 8);
-    return passes <= static_cast<int64_t>(g.cluster) * rows;
+    return passes <= static_cast<int64_t>(g.cluster) * kMostRows && g.batch * (g.vectors / g.slab) * g.cluster <= 4 * static_cast<int64_t>(sm_count());
 }
-constexpr int kMostRows = 16;      // rows of a thread that gcl_cluster keeps
 
 size_t up256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
 // the most any vector width asks for
@@ -503,13 +576,9 @@ struct GclCall {
 
 template <typename T, int V, bool WHOLE, int ACT>
 int run_cluster(const GclCall& c, const GclGeom& g, cudaStream_t s) {
-    const int64_t units = g.batch * ((g.vectors + g.slab - 1) / g.slab), passes = (g.spatial + g.rpp - 1) / g.rpp;
-    const int rows = static_cast<int>((passes + g.cluster - 1) / g.cluster);
-#define VRB_GCL_CLUSTER(R) launch_clusters(gcl_cluster_kernel<T, V, WHOLE, ACT, R>, static_cast<unsigned>(units * g.cluster), g.cluster, s, static_cast<const T*>(c.x), \
-                                           c.weight, c.w_dt, c.bias, c.b_dt, static_cast<T*>(c.out), g, c.eps, c.activation)
-    if (rows <= 4) VRB_GCL_CLUSTER(4);
-    else VRB_GCL_CLUSTER(kMostRows);
-#undef VRB_GCL_CLUSTER
+    const int64_t units = g.batch * ((g.vectors + g.slab - 1) / g.slab);
+    launch_clusters(gcl_cluster_kernel<T, V, WHOLE, ACT>, static_cast<unsigned>(units * g.cluster), g.cluster, s, static_cast<const T*>(c.x), c.weight, c.w_dt, c.bias,
+                    c.b_dt, static_cast<T*>(c.out), g, c.eps, c.activation);
     return after_launch("group_norm_channels_last");
 }
 template <typename T, int V, bool WHOLE>
@@ -528,7 +597,7 @@ int run_passes(const GclCall& c, GclGeom g, char* workspace, cudaStream_t s) {
     float2* stats = g.groups > kInlineGroups ? reinterpret_cast<float2*>(workspace + partial_bytes(g)) : nullptr;
     const dim3 ctas_stats(static_cast<unsigned>(g.batch * g.splits));
     const T* x = static_cast<const T*>(c.x);
-    if (g.per % V == 0) launch_overlapped(gcl_partial_kernel<T, V, true>, ctas_stats, dim3(kThreads), 0, s, x, partial, g);
+    if (one_group(g, V)) launch_overlapped(gcl_partial_kernel<T, V, true>, ctas_stats, dim3(kThreads), 0, s, x, partial, g);
     else if constexpr (V > 1 && V < 8) launch_overlapped(gcl_partial_kernel<T, V, false>, ctas_stats, dim3(kThreads), 0, s, x, partial, g);
     if (int rc = after_launch("group_norm_channels_last statistics")) return rc;
     if (stats) {
@@ -538,7 +607,7 @@ int run_passes(const GclCall& c, GclGeom g, char* workspace, cudaStream_t s) {
     }
     const int64_t slabs = (g.vectors + g.slab - 1) / g.slab, units = g.batch * slabs;
     int64_t ctas = (static_cast<int64_t>(sm_count()) * 2 + units - 1) / units;
-    const int64_t most = (g.spatial + g.rpp - 1) / g.rpp;
+    const int64_t most = (all_rows(g) + g.rpp - 1) / g.rpp;
     if (ctas > most) ctas = most;
     const dim3 grid(static_cast<unsigned>(units * ctas));
 #define VRB_GCL_APPLY(ACT) launch_overlapped(gcl_apply_kernel<T, V, ACT>, grid, dim3(kThreads), 0, s, static_cast<const T*>(c.x), c.weight, c.w_dt, c.bias, c.b_dt, \
@@ -554,9 +623,9 @@ int run_passes(const GclCall& c, GclGeom g, char* workspace, cudaStream_t s) {
 template <typename T, int V>
 int run_width(const GclCall& c, GclGeom g, bool cluster, char* workspace, cudaStream_t s) {
     if (!cluster) return run_passes<T, V>(c, g, workspace, s);
-    set_cluster(g, V, sizeof(T), kMostRows);
+    set_cluster(g, V, sizeof(T));
     if constexpr (V > 1 && V < 8)
-        if (g.per % V != 0) return run_cluster<T, V, false>(c, g, s);
+        if (!one_group(g, V)) return run_cluster<T, V, false>(c, g, s);
     return run_cluster<T, V, true>(c, g, s);
 }
 
@@ -573,7 +642,7 @@ extern "C" size_t vrb_group_norm_channels_last_workspace_bytes(int dtype, int64_
     bool cluster = true;
     for (int v = 16 / element; v >= 1 && cluster; v /= 2) {
         GclGeom h = g;
-        if (channels % v == 0 && (v < 8 || h.per % v == 0)) cluster = set_cluster(h, v, element, kMostRows);
+        if (channels % v == 0 && (v < 8 || groups == 1 || h.per % 8 == 0)) cluster = set_cluster(h, v, element);
     }
     return cluster ? 0 : workspace_size(g);
 }
@@ -590,9 +659,10 @@ extern "C" int vrb_group_norm_channels_last(const void* x, int dtype, const void
                 "group_norm_channels_last: unknown activation %d", activation);
     GclGeom g;
     if (int rc = make_geom(g, batch, spatial, channels, groups)) return rc;
-    const int v = vector_width(dtype, channels, groups, x, out);
+    int v = vector_width(dtype, batch, spatial, channels, groups, false, x, out);
     GclGeom h = g;
-    const bool cluster = set_cluster(h, v, static_cast<int>(dtype_bytes(dtype)), kMostRows);
+    const bool cluster = set_cluster(h, v, static_cast<int>(dtype_bytes(dtype)));
+    if (!cluster) v = vector_width(dtype, batch, spatial, channels, groups, true, x, out);
     const size_t need = cluster ? 0 : workspace_size(g);
     VRB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0), VRB_ERR_WORKSPACE,
                 "group_norm_channels_last: workspace needs %zu bytes, 256-byte aligned", need);
