@@ -19,7 +19,8 @@
 namespace vrb {
 namespace {
 
-constexpr int kThreads = 512;      // of the passes
+constexpr int kThreads = 512;      // of the statistics pass
+constexpr int kApplyThreads = 1024;// of the normalise pass: one CTA to an SM, so that the sums are added once on each
 constexpr int kClusterThreads = 256;
 constexpr int kRun = 32;           // rows of a thread between two rebuilds in double
 constexpr int kClusterGroups = 128;// groups of a cluster's slab, at most
@@ -206,7 +207,6 @@ __global__ void __launch_bounds__(kThreads, 1) gcl_partial_kernel(const T* x, do
     using Acc = Sums<T, V, WHOLE>;
     __shared__ double sums[2][kThreads * Acc::D];
     pdl_wait();
-    pdl_launch_dependents();   // gcl_apply reads x, weight and bias ahead of its own wait: all of them are there from here on
     const int b = blockIdx.x / g.splits, split = blockIdx.x - b * g.splits;
     const int lane_vector = threadIdx.x % g.slab, lane_row = threadIdx.x / g.slab;
     double* out = partial + static_cast<int64_t>(blockIdx.x) * g.groups * 2;
@@ -348,10 +348,11 @@ __device__ __forceinline__ void apply_stats(const GclGeom& g, int c0, Stat stat,
 
 // stats: finished, or nullptr: every CTA adds the CTAs' sums of its batch entry (groups <= kInlineGroups)
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads, 2) gcl_apply_kernel(const T* x, const void* weight, int w_dt, const void* bias, int b_dt, T* out,
+__global__ void __launch_bounds__(kApplyThreads, 1) gcl_apply_kernel(const T* x, const void* weight, int w_dt, const void* bias, int b_dt, T* out,
                                                                const double* __restrict__ partial, const float2* __restrict__ stats, GclGeom g, float eps,
                                                                int ctas, int kind) {
     __shared__ float2 own[kInlineGroups];
+    pdl_wait();
     const int slabs = (g.vectors + g.slab - 1) / g.slab;
     const int unit = blockIdx.x / ctas, cta = ctas - 1 - (blockIdx.x - unit * ctas);
     const int b = unit / slabs, slab0 = (unit - b * slabs) * g.slab;
@@ -360,25 +361,23 @@ __global__ void __launch_bounds__(kThreads, 2) gcl_apply_kernel(const T* x, cons
     const int c0 = (slab0 + lane_vector) * V, channel = g.fold > 1 ? c0 % g.row : c0;
     constexpr int U = 4;
     const int64_t step = static_cast<int64_t>(ctas) * g.rpp, p_step = step * g.channels;
-    // rows of this thread are cta * rpp + lane_row + i * step, visited from the last one down; the first U of them are on their
-    // way before the statistics are waited for (gcl_partial began after everything before it had ended)
-    const int64_t row0 = static_cast<int64_t>(cta) * g.rpp + lane_row;
-    int64_t row = row0 < g.spatial ? row0 + (g.spatial - 1 - row0) / step * step : -1;
-    int64_t at = b * g.entry + row * g.channels + c0;
-    Vec<T, V> v[U];
     float mean[V], scale[V], shift[V];
     if (live) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (row - u * step >= 0) v[u] = load_vec<true, T, V>(x + at - u * p_step);
         load_channels<V>(weight, w_dt, channel, g.row, 1.0f, scale);
         load_channels<V>(bias, b_dt, channel, g.row, 0.0f, shift);
     }
-    pdl_wait();
-    if (stats == nullptr) collect_groups<kThreads>(partial, b, 0, g.groups, g, eps, [&](int group, float2 v) { own[group] = v; });
+    if (stats == nullptr) collect_groups<kApplyThreads>(partial, b, 0, g.groups, g, eps, [&](int group, float2 v) { own[group] = v; });
     if (!live) return;
     apply_stats<V>(g, channel, [&](int group) { return stats ? stats[static_cast<int64_t>(b) * g.groups + group] : own[group]; }, mean, scale);
-    while (row >= 0) {
+    // rows of this thread are cta * rpp + lane_row + i * step, visited from the last one down
+    const int64_t row0 = static_cast<int64_t>(cta) * g.rpp + lane_row;
+    int64_t row = row0 < g.spatial ? row0 + (g.spatial - 1 - row0) / step * step : -1;
+    int64_t at = b * g.entry + row * g.channels + c0;
+    for (; row >= 0; row -= U * step, at -= U * p_step) {
+        Vec<T, V> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (row - u * step >= 0) v[u] = load_vec<true, T, V>(x + at - u * p_step);
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (row - u * step >= 0) {
@@ -387,11 +386,6 @@ __global__ void __launch_bounds__(kThreads, 2) gcl_apply_kernel(const T* x, cons
                 for (int e = 0; e < V; ++e) y[e] = activate<ACT>(fmaf(v[u].get(e) - mean[e], scale[e], shift[e]), kind);
                 store_vec<V>(out + at - u * p_step, y);
             }
-        row -= U * step;
-        at -= U * p_step;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (row - u * step >= 0) v[u] = load_vec<true, T, V>(x + at - u * p_step);
     }
     if (g.tail > 0 && row0 <= g.spatial && (g.spatial - row0) % step == 0) {
         constexpr int dt = sizeof(T) == 2 ? VRB_BF16 : VRB_F32;
@@ -605,12 +599,14 @@ int run_passes(const GclCall& c, GclGeom g, char* workspace, cudaStream_t s) {
                           stats, g, c.eps);
         if (int rc = after_launch("group_norm_channels_last finalize")) return rc;
     }
+    g.rpp = kApplyThreads / g.slab;
+    if (g.rpp > all_rows(g)) g.rpp = static_cast<int>(all_rows(g));
     const int64_t slabs = (g.vectors + g.slab - 1) / g.slab, units = g.batch * slabs;
-    int64_t ctas = (static_cast<int64_t>(sm_count()) * 2 + units - 1) / units;
+    int64_t ctas = (static_cast<int64_t>(sm_count()) + units - 1) / units;
     const int64_t most = (all_rows(g) + g.rpp - 1) / g.rpp;
     if (ctas > most) ctas = most;
     const dim3 grid(static_cast<unsigned>(units * ctas));
-#define VRB_GCL_APPLY(ACT) launch_overlapped(gcl_apply_kernel<T, V, ACT>, grid, dim3(kThreads), 0, s, static_cast<const T*>(c.x), c.weight, c.w_dt, c.bias, c.b_dt, \
+#define VRB_GCL_APPLY(ACT) launch_overlapped(gcl_apply_kernel<T, V, ACT>, grid, dim3(kApplyThreads), 0, s, static_cast<const T*>(c.x), c.weight, c.w_dt, c.bias, c.b_dt, \
                                              static_cast<T*>(c.out), partial, stats, g, c.eps, static_cast<int>(ctas), c.activation)
     if (c.activation == VRB_NO_ACTIVATION) VRB_GCL_APPLY(0);
     else if (c.activation == VRB_SILU) VRB_GCL_APPLY(1);
