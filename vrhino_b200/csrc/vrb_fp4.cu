@@ -6,16 +6,20 @@
 // word of the scale tile are collected by shuffles and leave as one 4-byte store.
 //
 // Rounding is that of the real quotients a / (6 g) -> e4m3 and x / (g s) -> e2m1.  The fast form multiplies by an F32
-// reciprocal (three roundings, relative error < 2^-22) and converts the product moved up and down by kGuard = 2^-21:
-// where both give one code it is the right one.  Where they differ a rounding border lies between, and the sign of
-// |x| - border * s * g, exact in double (at most 31 significant bits against 24), decides; 0 is the tie.
+// quotient (its 2 ulp and three roundings: relative error < 2^-21) and converts the product moved up and down by kGuard = 2^-20:
+// where both give one code it is the right one.  Where they differ a rounding border t lies between, and the sign of
+// |x| - t s g decides; 0 is the tie.  With s g = hi + lo in F32 (one product and one multiply-add, exact), |x| - t hi is exact
+// next to the border (the two agree to 20 bits) and the multiply-add with -t lo rounds to the right sign.  bf16 data meets
+// borders exactly (amax / 2688 = amax / (2^7 3 7) shares its factors with scales of 9, 12, 14 and 15 eighths): nearly every
+// warp takes this path for some element, so it goes element by element, in F32 (eight at a time in double: 99 us on
+// 13824 x 5120, this form 33).
 #include "vrb_fp4.cuh"
 
 namespace vrb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr float kGuard = 4.76837158203125e-7f;   // 2^-21
+constexpr float kGuard = 9.5367431640625e-7f;   // 2^-20
 
 // codes of 8 values, element 0 in the lowest nibble (e2m1: to nearest, ties to even, saturating)
 __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
@@ -59,13 +63,17 @@ __device__ __noinline__ uint32_t nv_scale_exact(float a, float g) {
     }
     return code < 126u ? code + 1u : 126u;
 }
-// one element, exactly: |x| against the borders times s g
+// the border above the magnitude of an e2m1 code: .25 .75 1.25 1.75 2.5 3.5 5
+__device__ __forceinline__ float e2m1_border(uint32_t magnitude) {
+    return 0.25f * static_cast<float>(e2m1_twice(magnitude) + e2m1_twice(magnitude + 1u));
+}
+// one element in double, for tensor scales outside the range of the F32 form
 __device__ __noinline__ uint32_t e2m1_exact(float x, double unit) {
     const uint32_t sign = __float_as_uint(x) >> 31 << 3;
     const double a = fabs(static_cast<double>(x));
     uint32_t code = 0;
     for (; code < 7u; ++code) {
-        const double border = 0.25 * static_cast<double>(e2m1_twice(code) + e2m1_twice(code + 1u)) * unit;
+        const double border = static_cast<double>(e2m1_border(code)) * unit;
         if (a < border || (a == border && (code & 1u) == 0u)) break;
     }
     return sign | code;
@@ -74,31 +82,99 @@ __device__ __noinline__ uint32_t e2m1_exact(float x, double unit) {
 template <typename T> struct Elements;
 template <> struct Elements<uint16_t> {
     static constexpr int kChunk = 8;     // elements of a 16-byte chunk
+    static constexpr int kWords = 8;     // words of 16 elements
     __device__ static __forceinline__ float value(uint16_t h) { return bf16_bits_to_float(h); }
 };
 template <> struct Elements<float> {
     static constexpr int kChunk = 4;
+    static constexpr int kWords = 16;
     __device__ static __forceinline__ float value(float f) { return f; }
 };
 
-// elements [column, column + 16) of a row of k, zero past the end
+// The words of elements [column, column + 16) of a row of k, zero past the end.  VEC: rows of whole 16-byte chunks on 16-byte boundaries.  Otherwise the 16 elements are cut out of the aligned
+// chunks around them by a shift of whole words and, bf16, of half a word; at the tensor's ends element by element.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load16(const T* row, int64_t column, int64_t k, float (&v)[16]) {
+__device__ __forceinline__ void load16(const T* x, int64_t count, const T* at, int64_t column, int64_t k, uint32_t (&w)[Elements<T>::kWords]) {
+    constexpr int W = Elements<T>::kWords;
+    const int live = k - column < 16 ? static_cast<int>(k - column) : 16;
     if constexpr (VEC) {
         constexpr int C = Elements<T>::kChunk;
 #pragma unroll
         for (int c = 0; c < 16 / C; ++c) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (column + c * C < k) w = __ldcs(reinterpret_cast<const uint4*>(row + column + c * C));
-            T e[C];
-            *reinterpret_cast<uint4*>(e) = w;
-#pragma unroll
-            for (int i = 0; i < C; ++i) v[c * C + i] = Elements<T>::value(e[i]);
+            uint4 q = make_uint4(0, 0, 0, 0);
+            if (c * C < live) q = __ldcs(reinterpret_cast<const uint4*>(at + c * C));
+            w[4 * c] = q.x; w[4 * c + 1] = q.y; w[4 * c + 2] = q.z; w[4 * c + 3] = q.w;
         }
     } else {
+        const uintptr_t address = reinterpret_cast<uintptr_t>(at), low = address & ~uintptr_t{15};
+        if (low >= reinterpret_cast<uintptr_t>(x) && low + (W + 4) * 4 <= reinterpret_cast<uintptr_t>(x + count)) {
+            uint32_t c[W + 4];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = column + i < k ? Elements<T>::value(row[column + i]) : 0.0f;
+            for (int i = 0; i < W / 4 + 1; ++i) {
+                const uint4 q = *reinterpret_cast<const uint4*>(low + i * 16);
+                c[4 * i] = q.x; c[4 * i + 1] = q.y; c[4 * i + 2] = q.z; c[4 * i + 3] = q.w;
+            }
+            const unsigned shift = static_cast<unsigned>(address & 15u);
+            if (shift & 8u)
+#pragma unroll
+                for (int i = 0; i < W + 2; ++i) c[i] = c[i + 2];
+            if (shift & 4u)
+#pragma unroll
+                for (int i = 0; i < W + 1; ++i) c[i] = c[i + 1];
+            const unsigned bits = (shift & 2u) * 8u;   // 0 for F32
+#pragma unroll
+            for (int i = 0; i < W; ++i) w[i] = sizeof(T) == 4 ? c[i] : __funnelshift_r(c[i], c[i + 1], bits);
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) w[i] = 0u;
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (i < live) w[i] = __float_as_uint(at[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (i < live) w[i / 2] |= static_cast<uint32_t>(at[i]) << (i % 2 * 16);
+            }
+        }
+        if (live < 16) {   // what follows the row's end belongs to the next row
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                if constexpr (sizeof(T) == 4) w[i] = i < live ? w[i] : 0u;
+                else w[i] = 2 * i + 1 < live ? w[i] : 2 * i < live ? w[i] & 0xffffu : 0u;
+            }
+        }
     }
+}
+// The elements as F32, and the bits of the largest magnitude (a NaN's are above every other's)
+template <typename T>
+__device__ __forceinline__ uint32_t values16(const uint32_t (&w)[Elements<T>::kWords], float (&v)[16]) {
+    constexpr int W = Elements<T>::kWords;
+    uint32_t top;
+    if constexpr (sizeof(T) == 2) {
+        top = w[0] & 0x7fff7fffu;
+#pragma unroll
+        for (int i = 1; i < W; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+        top = max(top << 16, top & 0xffff0000u);
+#pragma unroll
+        for (int i = 0; i < W; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    } else {
+        top = 0u;
+#pragma unroll
+        for (int i = 0; i < W; ++i) { v[i] = __uint_as_float(w[i]); top = max(top, w[i] & 0x7fffffffu); }
+    }
+    return top;
+}
+// v[i] of eight registers
+__device__ __forceinline__ float pick8(const float* v, int i) {
+    const float a = i & 1 ? v[1] : v[0], b = i & 1 ? v[3] : v[2], c = i & 1 ? v[5] : v[4], d = i & 1 ? v[7] : v[6];
+    const float ab = i & 2 ? b : a, cd = i & 2 ? d : c;
+    return i & 4 ? cd : ab;
+}
+__device__ __forceinline__ void scale8(const float* v, float r, float (&y)[8]) {
+    const unsigned long long rr = pack_f32x2(r, r);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) unpack_f32x2(mul_f32x2(pack_f32x2(v[i], v[i + 1]), rr), y[i], y[i + 1]);
 }
 
 struct PackGeom {
@@ -108,95 +184,134 @@ struct PackGeom {
     int64_t tile_row;      // bytes of a row of scale tiles
 };
 
-template <typename T, int FORMAT, bool VEC>
+// LANES threads share a word of the scale tile (a segment of 16 elements each); 1: a thread takes all of a word's segments in
+// turn, for rows so short that most segments of a word are padding.
+template <typename T, int FORMAT, bool VEC, int LANES>
 __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const T* __restrict__ x, const float* tensor_scale, uint8_t* __restrict__ codes,
                                                                uint8_t* __restrict__ scales, PackGeom p) {
+    constexpr int kPerWord = FORMAT == VRB_NVFP4 ? 4 : 8;      // segments of a scale word
+    constexpr int kSerial = LANES == 1 ? kPerWord : 1;
     pdl_wait();
     const float g = FORMAT == VRB_NVFP4 && tensor_scale ? *tensor_scale : 1.0f;
     // 2^-100 .. 2^100: the F32 form neither overflows nor loses bits below the normal range
     const bool fast = g >= 7.888609052210118e-31f && g <= 1.2676506002282294e30f;
-    const int64_t total = p.padded_rows * p.segments, stride = static_cast<int64_t>(gridDim.x) * kThreads;
+    const float g6 = __fmul_rn(6.0f, g);
+    const int64_t units = p.segments / kSerial;                // of a row
+    const int64_t total = p.padded_rows * units, stride = static_cast<int64_t>(gridDim.x) * kThreads;
     int64_t u = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-    const int64_t d_row = stride / p.segments, d_segment = stride - d_row * p.segments;
-    int64_t row = u / p.segments, segment = u - row * p.segments;
+    const int64_t d_row = stride / units, d_unit = stride - d_row * units;
+    int64_t row = u / units, unit = u - row * units;
     const int lane = threadIdx.x & 31;
-    // total and stride are multiples of the 4 or 8 segments that share a scale word, so those lanes stay together
-    for (; u < total; u += stride) {
-        const int64_t warp_left = total - (u - lane);
-        const unsigned group = warp_left >= 32 ? 0xffffffffu : (1u << warp_left) - 1u;   // lanes that hold a segment
-        const int64_t column = segment * 16;
-        float v[16];
-        const bool live = row < p.rows && column < p.k;
-        if (live) load16<T, VEC>(x + row * p.k, column, p.k, v);
+    const int64_t count = p.rows * p.k;
+    auto fetch = [&](int64_t r, int64_t column, uint32_t (&w)[Elements<T>::kWords]) {
+        if (r < p.rows && column < p.k) load16<T, VEC>(x, count, x + r * p.k + column, column, p.k, w);
         else
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = 0.0f;
-        uint32_t top = 0;   // bits of the largest magnitude; a NaN is above everything
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-        if constexpr (FORMAT == VRB_MXFP4) top = max(top, __shfl_xor_sync(group, top, 1));
-        uint32_t byte, word0 = 0, word1 = 0;
-        if constexpr (FORMAT == VRB_NVFP4) {
-            const float a = __uint_as_float(top);
-            if (top >= 0x7f800000u || !(g <= 3.402823466e38f)) {
-                byte = 0x7fu;
-            } else if (top == 0u || g == 0.0f) {
-                byte = 0u;
+            for (int i = 0; i < Elements<T>::kWords; ++i) w[i] = 0u;
+    };
+    uint32_t ahead[Elements<T>::kWords];
+    if constexpr (LANES > 1)
+        if (u < total) fetch(row, unit * 16, ahead);
+    // total and stride are multiples of the lanes that share a scale word, so those stay together
+    for (; u < total; u += stride) {
+        const int64_t warp_left = total - (u - lane);
+        const unsigned group = warp_left >= 32 ? 0xffffffffu : (1u << warp_left) - 1u;   // lanes that hold a unit
+        int64_t next_row = row + d_row, next_unit = unit + d_unit;
+        if (next_unit >= units) { next_unit -= units; ++next_row; }
+        uint32_t word = 0u, carried = 0u;
+#pragma unroll 1
+        for (int part = 0; part < kSerial; ++part) {
+            const int64_t segment = unit * kSerial + part, column = segment * 16;
+            float v[16];
+            uint32_t top;
+            if constexpr (LANES > 1) {   // the next unit's elements are on their way while this one's are packed
+                top = values16<T>(ahead, v);
+                if (u + stride < total) fetch(next_row, next_unit * 16, ahead);
             } else {
-                const float q = __fdiv_rn(a, __fmul_rn(6.0f, g));
-                const uint32_t lo = e4m3_bits(q * (1.0f - kGuard)), hi = e4m3_bits(q * (1.0f + kGuard));
-                byte = fast && lo == hi ? lo : nv_scale_exact(a, g);
+                uint32_t w[Elements<T>::kWords];
+                fetch(row, column, w);
+                top = values16<T>(w, v);
             }
-            if (byte != 0u && byte != 0x7fu) {
-                const float s = e4m3_value(byte);
-                const double unit = static_cast<double>(s) * static_cast<double>(g);
-                const float r = __fdiv_rn(1.0f, __fmul_rn(s, g)), r_lo = r * (1.0f - kGuard), r_hi = r * (1.0f + kGuard);
+            const bool live = row < p.rows && column < p.k;
+            uint32_t byte = 0u, word0 = 0u, word1 = 0u;
+            if constexpr (FORMAT == VRB_NVFP4) {
+                const float a = __uint_as_float(top);
+                if (top >= 0x7f800000u || !(g <= 3.402823466e38f)) {
+                    byte = live ? 0x7fu : 0u;
+                } else if (top != 0u && g != 0.0f) {
+                    const float q = __fdividef(a, g6);
+                    const uint32_t lo = e4m3_bits(q * (1.0f - kGuard)), hi = e4m3_bits(q * (1.0f + kGuard));
+                    byte = fast && lo == hi ? lo : nv_scale_exact(a, g);
+                }
+                if (byte != 0u && byte != 0x7fu) {
+                    const float s = e4m3_value(byte), hi = __fmul_rn(s, g), lo = __fmaf_rn(s, g, -hi);
+                    const float r = __fdividef(1.0f, hi);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float lo[8], hi[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) { lo[i] = v[h * 8 + i] * r_lo; hi[i] = v[h * 8 + i] * r_hi; }
-                    uint32_t w = e2m1x8(lo);
-                    if (!fast || w != e2m1x8(hi)) {
-                        w = 0;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) w |= e2m1_exact(v[h * 8 + i], unit) << (4 * i);
+                    for (int h = 0; h < 2; ++h) {
+                        float y[8];
+                        scale8(v + h * 8, r * (1.0f - kGuard), y);
+                        uint32_t w = e2m1x8(y);
+                        scale8(v + h * 8, r * (1.0f + kGuard), y);
+                        uint32_t differ = e2m1x8(y) ^ w;
+                        if (!fast) {
+                            w = 0u;
+#pragma unroll 1
+                            for (int i = 0; i < 8; ++i) w |= e2m1_exact(pick8(v + h * 8, i), static_cast<double>(s) * static_cast<double>(g)) << (4 * i);
+                            differ = 0u;
+                        }
+                        while (differ != 0u) {   // elements next to a border; w has the code below it
+                            const int i = (__ffs(differ) - 1) >> 2;
+                            differ &= ~(15u << (4 * i));
+                            const uint32_t code = w >> (4 * i) & 7u;
+                            const float t = e2m1_border(code);
+                            const float d = __fmaf_rn(-t, lo, __fmaf_rn(-t, hi, fabsf(pick8(v + h * 8, i))));
+                            if (d > 0.0f || (d == 0.0f && (code & 1u) != 0u)) w += 1u << (4 * i);
+                        }
+                        (h ? word1 : word0) = w;
                     }
-                    (h ? word1 : word0) = w;
                 }
-            }
-        } else {
-            if (top >= 0x7f800000u) {
-                byte = 0xffu;
             } else {
-                const int e = static_cast<int>(top >> 23) - 2;   // biased exponent of 2^(floor(log2 a) - 2)
-                byte = e > 0 ? static_cast<uint32_t>(e) : 0u;
-                const float r = __uint_as_float((254u - byte) << 23);   // 2^(127 - byte): the product is exact or far below the first border
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float q[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) q[i] = v[h * 8 + i] * r;
-                    (h ? word1 : word0) = e2m1x8(q);
+                // the block's two halves: neighbouring lanes, or this thread's last and next segment
+                if constexpr (LANES > 1) {
+                    top = max(top, __shfl_xor_sync(group, top, 1));
+                } else {
+                    uint32_t w[Elements<T>::kWords];
+                    float other[16];
+                    fetch(row, column ^ 16, w);
+                    top = max(top, values16<T>(w, other));
+                }
+                if (top >= 0x7f800000u) {
+                    byte = 0xffu;
+                } else {
+                    const int e = static_cast<int>(top >> 23) - 2;   // biased exponent of 2^(floor(log2 a) - 2)
+                    byte = e > 0 ? static_cast<uint32_t>(e) : 0u;
+                    const float r = __uint_as_float((254u - byte) << 23);   // 2^(127 - byte): the product is exact or far below the first border
+                    float y[8];
+                    scale8(v, r, y);
+                    word0 = e2m1x8(y);
+                    scale8(v + 8, r, y);
+                    word1 = e2m1x8(y);
                 }
             }
-            if (top == 0u) byte = 0u;
+            if (row < p.rows && segment * 8 < p.row_bytes)
+                *reinterpret_cast<uint2*>(codes + row * p.row_bytes + segment * 8) = make_uint2(word0, word1);
+            constexpr int kPerBlock = FORMAT == VRB_NVFP4 ? 1 : 2;   // segments of a block
+            const bool in_block = row < p.rows && (FORMAT == VRB_NVFP4 ? column < p.k : (segment & ~int64_t{1}) * 16 < p.k);
+            word = in_block ? byte : 0u;
+            if constexpr (LANES > 1) {
+                word |= __shfl_xor_sync(group, word, kPerBlock) << 8;
+                word |= __shfl_xor_sync(group, word, 2 * kPerBlock) << 16;
+            } else {
+                carried |= word << (part / kPerBlock * 8);
+            }
         }
-        if (row < p.rows && segment * 8 < p.row_bytes)
-            *reinterpret_cast<uint2*>(codes + row * p.row_bytes + segment * 8) = make_uint2(word0, word1);
-        // four consecutive blocks make a word of the scale tile
-        constexpr int kLanes = FORMAT == VRB_NVFP4 ? 1 : 2;   // lanes of a block
-        const bool in_block = FORMAT == VRB_NVFP4 ? column < p.k : (segment & ~int64_t{1}) * 16 < p.k;
-        uint32_t word = row < p.rows && in_block ? byte : 0u;
-        word |= __shfl_xor_sync(group, word, kLanes) << 8;
-        word |= __shfl_xor_sync(group, word, 2 * kLanes) << 16;
-        if ((segment & (4 * kLanes - 1)) == 0) {
-            const int64_t at = (row >> 7) * p.tile_row + segment / (4 * kLanes) * 512 + (row & 31) * 16 + ((row & 127) >> 5) * 4;
-            *reinterpret_cast<uint32_t*>(scales + at) = word;
+        if (LANES == 1 || (unit & (kPerWord - 1)) == 0) {
+            const int64_t word_index = LANES == 1 ? unit : unit / kPerWord;
+            const int64_t at = (row >> 7) * p.tile_row + word_index * 512 + (row & 31) * 16 + ((row & 127) >> 5) * 4;
+            *reinterpret_cast<uint32_t*>(scales + at) = LANES == 1 ? carried : word;
         }
-        row += d_row;
-        segment += d_segment;
-        if (segment >= p.segments) { segment -= p.segments; ++row; }
+        row = next_row;
+        unit = next_unit;
     }
 }
 
@@ -207,55 +322,82 @@ __device__ __forceinline__ void e2m1x2_values(uint32_t byte, float& lo, float& h
     asm("{\n\t.reg .b16 l, u;\n\tmov.b32 {l, u}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, u;\n\t}" : "=f"(lo), "=f"(hi) : "r"(h));
 }
 
+// A thread writes 16 elements that begin on a 16-byte boundary of the result.  Rows of whole chunks (VEC): one segment.
+// Otherwise a row that begins `phase` elements past a boundary is cut into windows of columns [16 w - phase, 16 w - phase + 16):
+// the codes of two segments joined by a shift and up to two scales; windows over a row's ends go element by element.
+template <int FORMAT>
+__device__ __forceinline__ float scale_of(const uint8_t* scales, const PackGeom& p, int64_t row, int64_t segment) {
+    const int64_t block = FORMAT == VRB_NVFP4 ? segment : segment >> 1;
+    const uint32_t byte = scales[(row >> 7) * p.tile_row + (block >> 2) * 512 + (row & 31) * 16 + ((row & 127) >> 5) * 4 + (block & 3)];
+    if constexpr (FORMAT == VRB_NVFP4) return byte == 0x7fu ? __uint_as_float(0x7fffffffu) : e4m3_value(byte);
+    else return byte == 0xffu ? __uint_as_float(0x7fffffffu) : __uint_as_float(byte ? byte << 23 : 0x00400000u);
+}
 template <typename T, int FORMAT, bool VEC>
 __global__ void __launch_bounds__(kThreads) fp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                                  const float* tensor_scale, T* __restrict__ out, PackGeom p) {
+    constexpr int kPhases = Elements<T>::kChunk;
     pdl_wait();
     const float g = FORMAT == VRB_NVFP4 && tensor_scale ? *tensor_scale : 1.0f;
-    const int64_t segments = (p.k + 15) / 16;
-    const int64_t total = p.rows * segments, stride = static_cast<int64_t>(gridDim.x) * kThreads;
+    const int64_t windows = VEC ? (p.k + 15) / 16 : (p.k + kPhases - 1 + 15) / 16;
+    const int64_t total = p.rows * windows, stride = static_cast<int64_t>(gridDim.x) * kThreads;
     int64_t u = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-    const int64_t d_row = stride / segments, d_segment = stride - d_row * segments;
-    int64_t row = u / segments, segment = u - row * segments;
+    const int64_t d_row = stride / windows, d_window = stride - d_row * windows;
+    int64_t row = u / windows, window = u - row * windows;
+    const int offset = static_cast<int>(reinterpret_cast<uintptr_t>(out) % 16 / sizeof(T));
     for (; u < total; u += stride) {
-        const uint2 w = __ldcs(reinterpret_cast<const uint2*>(codes + row * p.row_bytes + segment * 8));
-        const int64_t block = FORMAT == VRB_NVFP4 ? segment : segment >> 1;
-        const uint32_t byte = scales[(row >> 7) * p.tile_row + (block >> 2) * 512 + (row & 31) * 16 + ((row & 127) >> 5) * 4 + (block & 3)];
-        float s;
-        if constexpr (FORMAT == VRB_NVFP4) s = byte == 0x7fu ? __uint_as_float(0x7fffffffu) : e4m3_value(byte);
-        else s = byte == 0xffu ? __uint_as_float(0x7fffffffu) : __uint_as_float(byte ? byte << 23 : 0x00400000u);
-        float v[16];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            e2m1x2_values(((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 0xffu, v[2 * i], v[2 * i + 1]);
-            v[2 * i] = __fmul_rn(__fmul_rn(v[2 * i], s), g);
-            v[2 * i + 1] = __fmul_rn(__fmul_rn(v[2 * i + 1], s), g);
-        }
-        T* o = out + row * p.k + segment * 16;
-        if constexpr (VEC) {   // k % 16 == 0
-            if constexpr (sizeof(T) == 2) {
-                store16_bf16(out, row * p.k + segment * 16, v);
-            } else {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float y[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) y[i] = v[h * 8 + i];
-                    store8(out, VRB_F32, row * p.k + segment * 16 + h * 8, y);
+        const int phase = VEC ? 0 : static_cast<int>(static_cast<uint64_t>(row * p.k + offset) & (kPhases - 1));
+        const int64_t column = window * 16 - phase;
+        if (VEC || column < p.k) {
+            const uint8_t* row_codes = codes + row * p.row_bytes;
+            const int64_t last = (p.k - 1) / 16;               // segments of the row that hold elements
+            uint64_t bits = 0;
+            float s_lo = 0.0f, s_hi = 0.0f;                    // of the elements before and from `phase` on
+            if (window <= last) {
+                bits = __ldcs(reinterpret_cast<const unsigned long long*>(row_codes + window * 8));
+                s_hi = scale_of<FORMAT>(scales, p, row, window);
+            }
+            if constexpr (!VEC) {
+                if (phase > 0) {
+                    bits <<= 4 * phase;
+                    if (window > 0) {
+                        bits |= *reinterpret_cast<const unsigned long long*>(row_codes + (window - 1) * 8) >> (64 - 4 * phase);
+                        s_lo = scale_of<FORMAT>(scales, p, row, window - 1);
+                    }
                 }
             }
-        } else {
-            const int n = static_cast<int>(p.k - segment * 16 < 16 ? p.k - segment * 16 : 16);
+            float v[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (i < n) {
-                    if constexpr (sizeof(T) == 2) o[i] = static_cast<uint16_t>(float_to_bf16_bits(v[i]));
-                    else o[i] = v[i];
+            for (int i = 0; i < 8; ++i) {
+                e2m1x2_values(static_cast<uint32_t>(bits >> (8 * i)) & 0xffu, v[2 * i], v[2 * i + 1]);
+                const float s0 = !VEC && 2 * i < phase ? s_lo : s_hi, s1 = !VEC && 2 * i + 1 < phase ? s_lo : s_hi;
+                v[2 * i] = __fmul_rn(__fmul_rn(v[2 * i], s0), g);
+                v[2 * i + 1] = __fmul_rn(__fmul_rn(v[2 * i + 1], s1), g);
+            }
+            const int64_t at = row * p.k + column;
+            if (VEC || (column >= 0 && column + 16 <= p.k)) {
+                if constexpr (sizeof(T) == 2) {
+                    store16_bf16(out, at, v);
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float y[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) y[i] = v[h * 8 + i];
+                        store8(out, VRB_F32, at + h * 8, y);
+                    }
                 }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (column + i >= 0 && column + i < p.k) {
+                        if constexpr (sizeof(T) == 2) out[at + i] = static_cast<uint16_t>(float_to_bf16_bits(v[i]));
+                        else out[at + i] = v[i];
+                    }
+            }
         }
         row += d_row;
-        segment += d_segment;
-        if (segment >= segments) { segment -= segments; ++row; }
+        window += d_window;
+        if (window >= windows) { window -= windows; ++row; }
     }
 }
 
@@ -275,18 +417,20 @@ __global__ void __launch_bounds__(kThreads) fp4_tensor_scale_kernel(const T* __r
     if (tid < head) take(x[tid]);
     const T* body = x + head;
     const int64_t chunks = (count - head) / C;
-    for (int64_t i = tid; i < chunks; i += 4 * stride) {
-        uint4 w[4];
+    for (int64_t i = tid; i < chunks; i += 8 * stride) {
+        uint4 w[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 8; ++j)
             if (i + j * stride < chunks) w[j] = *reinterpret_cast<const uint4*>(body + (i + j * stride) * C);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 8; ++j)
             if (i + j * stride < chunks) {
-                T e[C];
-                *reinterpret_cast<uint4*>(e) = w[j];
-#pragma unroll
-                for (int k = 0; k < C; ++k) take(e[k]);
+                if constexpr (sizeof(T) == 2) {
+                    const uint32_t two = __vmaxu2(__vmaxu2(w[j].x & 0x7fff7fffu, w[j].y & 0x7fff7fffu), __vmaxu2(w[j].z & 0x7fff7fffu, w[j].w & 0x7fff7fffu));
+                    top = max(top, max(two << 16, two & 0xffff0000u));
+                } else {
+                    top = max(top, max(max(w[j].x & 0x7fffffffu, w[j].y & 0x7fffffffu), max(w[j].z & 0x7fffffffu, w[j].w & 0x7fffffffu)));
+                }
             }
     }
     if (tid < count - head - chunks * C) take(body[chunks * C + tid]);
@@ -334,7 +478,7 @@ extern "C" int vrb_fp4_tensor_scale(const void* x, int dtype, int64_t count, flo
     const int64_t element = static_cast<int64_t>(dtype_bytes(dtype));
     int64_t head = (16 - static_cast<int64_t>(reinterpret_cast<uintptr_t>(x) & 15u)) % 16 / element;
     if (head > count) head = count;
-    const int grid = grid_for((count / (16 / element) + kThreads * 4 - 1) / (kThreads * 4), 8);
+    const int grid = grid_for((count / (16 / element) + kThreads * 8 - 1) / (kThreads * 8), 4);
     if (dtype == VRB_BF16) launch_overlapped(fp4_tensor_scale_kernel<uint16_t>, dim3(grid), dim3(kThreads), 0, s, static_cast<const uint16_t*>(x), count, head, tensor_scale);
     else launch_overlapped(fp4_tensor_scale_kernel<float>, dim3(grid), dim3(kThreads), 0, s, static_cast<const float*>(x), count, head, tensor_scale);
     return after_launch("fp4_tensor_scale");
@@ -348,15 +492,18 @@ extern "C" int vrb_fp4_quantize(int format, const void* x, int dtype, const floa
     if (int rc = make_pack(p, format, rows, k, "fp4_quantize")) return rc;
     VRB_REQUIRE(format == VRB_NVFP4 || !tensor_scale, VRB_ERR_INVALID, "fp4_quantize: MXFP4 has no tensor scale");
     VRB_REQUIRE(aligned16(codes) && aligned16(scales), VRB_ERR_INVALID, "fp4_quantize: codes and scales must be 16-byte aligned");
-    const int64_t units = p.padded_rows * p.segments;
+    // a thread to a scale word where the rows have one and at most half of its segments hold elements
+    const bool serial = p.tile_row == 512 && k <= p.segments * 16 / 2;
+    const int64_t units = p.padded_rows * (serial ? 1 : p.segments);
     const dim3 grid(static_cast<unsigned>(grid_for((units + kThreads - 1) / kThreads, 8)));
     const bool vec = aligned16(x) && k % (16 / static_cast<int64_t>(dtype_bytes(dtype))) == 0;
     cudaStream_t s = as_stream(stream);
-#define VRB_PACK(T, F, V) launch_overlapped(fp4_quantize_kernel<T, F, V>, grid, dim3(kThreads), 0, s, static_cast<const T*>(x), tensor_scale, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), p)
-#define VRB_PACK_T(T) do { if (format == VRB_NVFP4) { if (vec) VRB_PACK(T, VRB_NVFP4, true); else VRB_PACK(T, VRB_NVFP4, false); } \
-                           else { if (vec) VRB_PACK(T, VRB_MXFP4, true); else VRB_PACK(T, VRB_MXFP4, false); } } while (0)
+#define VRB_PACK(T, F, V, L) launch_overlapped(fp4_quantize_kernel<T, F, V, L>, grid, dim3(kThreads), 0, s, static_cast<const T*>(x), tensor_scale, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), p)
+#define VRB_PACK_F(T, F, L) do { if (serial) VRB_PACK(T, F, false, 1); else if (vec) VRB_PACK(T, F, true, L); else VRB_PACK(T, F, false, L); } while (0)
+#define VRB_PACK_T(T) do { if (format == VRB_NVFP4) VRB_PACK_F(T, VRB_NVFP4, 4); else VRB_PACK_F(T, VRB_MXFP4, 8); } while (0)
     if (dtype == VRB_BF16) VRB_PACK_T(uint16_t); else VRB_PACK_T(float);
 #undef VRB_PACK_T
+#undef VRB_PACK_F
 #undef VRB_PACK
     return after_launch("fp4_quantize");
 }
@@ -369,7 +516,7 @@ extern "C" int vrb_fp4_dequantize(int format, const void* codes, const void* sca
     if (int rc = make_pack(p, format, rows, k, "fp4_dequantize")) return rc;
     VRB_REQUIRE(format == VRB_NVFP4 || !tensor_scale, VRB_ERR_INVALID, "fp4_dequantize: MXFP4 has no tensor scale");
     VRB_REQUIRE(aligned16(codes) && aligned16(scales), VRB_ERR_INVALID, "fp4_dequantize: codes and scales must be 16-byte aligned");
-    const int64_t units = rows * ((k + 15) / 16);
+    const int64_t units = rows * ((k + 15) / 16 + 1);
     const dim3 grid(static_cast<unsigned>(grid_for((units + kThreads - 1) / kThreads, 8)));
     const bool vec = aligned16(out) && k % 16 == 0;
     cudaStream_t s = as_stream(stream);
