@@ -7,12 +7,13 @@
 //
 // Rounding is that of the real quotients a / (6 g) -> e4m3 and x / (g s) -> e2m1.  The fast form multiplies by an F32
 // quotient (its 2 ulp and three roundings: relative error < 2^-21) and converts the product moved up and down by kGuard = 2^-20:
-// where both give one code it is the right one.  Where they differ a rounding border t lies between, and the sign of
-// |x| - t s g decides; 0 is the tie.  With s g = hi + lo in F32 (one product and one multiply-add, exact), |x| - t hi is exact
-// next to the border (the two agree to 20 bits) and the multiply-add with -t lo rounds to the right sign.  bf16 data meets
-// borders exactly (amax / 2688 = amax / (2^7 3 7) shares its factors with scales of 9, 12, 14 and 15 eighths): nearly every
-// warp takes this path for some element, so it goes element by element, in F32 (eight at a time in double: 99 us on
-// 13824 x 5120, this form 33).
+// where both give one code it is the right one.  Where they differ a rounding border t lies between, and eight elements are
+// done again (refined8): with s g = hi + lo in F32 (one product and one multiply-add, exact) a residual step gives the quotient
+// y to within an F32 step, so y is on t's right side unless it is t itself; then |x| - t hi is exact and a multiply-add with
+// -t lo rounds to the right sign, which moves y off the border; 0 is the tie.  bf16 data meets the borders of NVFP4 to within
+// 2^-24 all the time (the tensor scale is amax / (2^7 3 7), whose factors the scales 9, 12, 14 and 15 eighths share), and more
+// or less of it with amax, so the second form has no loop over elements: 13824 x 5120 bf16 took 99 us with a search in double
+// and 36 to 78, by amax, with a loop over the elements concerned.
 #include "vrb_fp4.cuh"
 
 namespace vrb {
@@ -44,12 +45,6 @@ __device__ __forceinline__ float e4m3_value(uint32_t code) {
     const uint32_t e = code >> 3, m = code & 7u;
     return e ? __uint_as_float(((e + 120u) << 23) | (m << 20)) : static_cast<float>(m) * 0.001953125f;   // 2^-9
 }
-// 2 * magnitude of an e2m1 code: 0 1 2 3 4 6 8 12
-__device__ __forceinline__ int e2m1_twice(uint32_t code) {
-    const uint32_t m = code & 7u;
-    return m < 4u ? static_cast<int>(m) : static_cast<int>((2u + (m & 1u)) << (m / 2u - 1u));
-}
-
 // Scale byte of an NVFP4 block with largest magnitude a: RN_e4m3(min(a / (6 g), 448))
 __device__ __noinline__ uint32_t nv_scale_exact(float a, float g) {
     // the quotient in double keeps its side of every border: borders have 5 significant bits, 6 g has 27, so the quotient
@@ -63,17 +58,13 @@ __device__ __noinline__ uint32_t nv_scale_exact(float a, float g) {
     }
     return code < 126u ? code + 1u : 126u;
 }
-// the border above the magnitude of an e2m1 code: .25 .75 1.25 1.75 2.5 3.5 5
-__device__ __forceinline__ float e2m1_border(uint32_t magnitude) {
-    return 0.25f * static_cast<float>(e2m1_twice(magnitude) + e2m1_twice(magnitude + 1u));
-}
 // one element in double, for tensor scales outside the range of the F32 form
 __device__ __noinline__ uint32_t e2m1_exact(float x, double unit) {
     const uint32_t sign = __float_as_uint(x) >> 31 << 3;
     const double a = fabs(static_cast<double>(x));
     uint32_t code = 0;
     for (; code < 7u; ++code) {
-        const double border = static_cast<double>(e2m1_border(code)) * unit;
+        const double border = 0.25 * static_cast<double>(0x140e0a0705030100ull >> (8u * code + 8u) & 0xffu) * unit;   // .25 .75 1.25 1.75 2.5 3.5 5
         if (a < border || (a == border && (code & 1u) == 0u)) break;
     }
     return sign | code;
@@ -171,6 +162,27 @@ __device__ __forceinline__ float pick8(const float* v, int i) {
     const float ab = i & 2 ? b : a, cd = i & 2 ? d : c;
     return i & 4 ? cd : ab;
 }
+// y / (hi + lo) of eight values to within an F32 step, moved off a value of three significant bits (the borders among them) to the
+// side the exact quotient lies on; r ~ 1 / hi
+__device__ __forceinline__ void refined8(const float* v, float hi, float lo, float r, float (&y)[8]) {
+    const unsigned long long nh = pack_f32x2(-hi, -hi), nl = pack_f32x2(-lo, -lo), rr = pack_f32x2(r, r);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const unsigned long long x = pack_f32x2(v[i], v[i + 1]);
+        unsigned long long q = mul_f32x2(x, rr);
+        q = fma_f32x2(fma_f32x2(q, nl, fma_f32x2(q, nh, x)), rr, q);
+        const unsigned long long rest = fma_f32x2(q, nl, fma_f32x2(q, nh, x));
+        float q0, q1, e0, e1;
+        unpack_f32x2(q, q0, q1);
+        unpack_f32x2(rest, e0, e1);
+        auto move = [](float a, float e, float of) {
+            const int bits = __float_as_int(a) | (__float_as_int(of) & 0x80000000), step = ((__float_as_int(e) ^ bits) >> 31) | 1;   // -1: the quotient is nearer to 0
+            return __int_as_float((bits & 0x1fffff) == 0 && e != 0.0f ? bits + step : bits);
+        };
+        y[i] = move(q0, e0, v[i]);           // the sign of -0 is lost on the way
+        y[i + 1] = move(q1, e1, v[i + 1]);
+    }
+}
 __device__ __forceinline__ void scale8(const float* v, float r, float (&y)[8]) {
     const unsigned long long rr = pack_f32x2(r, r);
 #pragma unroll
@@ -240,8 +252,14 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const T* __restr
                     byte = live ? 0x7fu : 0u;
                 } else if (top != 0u && g != 0.0f) {
                     const float q = __fdividef(a, g6);
-                    const uint32_t lo = e4m3_bits(q * (1.0f - kGuard)), hi = e4m3_bits(q * (1.0f + kGuard));
-                    byte = fast && lo == hi ? lo : nv_scale_exact(a, g);
+                    byte = e4m3_bits(q * (1.0f - kGuard));
+                    if (!fast) {
+                        byte = nv_scale_exact(a, g);
+                    } else if (byte != e4m3_bits(q * (1.0f + kGuard))) {   // next to a border: as for the elements, 6 g = g6 + its rest
+                        const float border = 0.5f * (e4m3_value(byte) + e4m3_value(byte + 1u));
+                        const float d = __fmaf_rn(-border, __fmaf_rn(6.0f, g, -g6), __fmaf_rn(-border, g6, a));
+                        byte += d > 0.0f || (d == 0.0f && (byte & 1u) != 0u) ? 1u : 0u;
+                    }
                 }
                 if (byte != 0u && byte != 0x7fu) {
                     const float s = e4m3_value(byte), hi = __fmul_rn(s, g), lo = __fmaf_rn(s, g, -hi);
@@ -252,20 +270,14 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const T* __restr
                         scale8(v + h * 8, r * (1.0f - kGuard), y);
                         uint32_t w = e2m1x8(y);
                         scale8(v + h * 8, r * (1.0f + kGuard), y);
-                        uint32_t differ = e2m1x8(y) ^ w;
+                        const uint32_t above = e2m1x8(y);
                         if (!fast) {
                             w = 0u;
 #pragma unroll 1
                             for (int i = 0; i < 8; ++i) w |= e2m1_exact(pick8(v + h * 8, i), static_cast<double>(s) * static_cast<double>(g)) << (4 * i);
-                            differ = 0u;
-                        }
-                        while (differ != 0u) {   // elements next to a border; w has the code below it
-                            const int i = (__ffs(differ) - 1) >> 2;
-                            differ &= ~(15u << (4 * i));
-                            const uint32_t code = w >> (4 * i) & 7u;
-                            const float t = e2m1_border(code);
-                            const float d = __fmaf_rn(-t, lo, __fmaf_rn(-t, hi, fabsf(pick8(v + h * 8, i))));
-                            if (d > 0.0f || (d == 0.0f && (code & 1u) != 0u)) w += 1u << (4 * i);
+                        } else if (w != above) {
+                            refined8(v + h * 8, hi, lo, r, y);
+                            w = e2m1x8(y);
                         }
                         (h ? word1 : word0) = w;
                     }

@@ -15,8 +15,8 @@ Every call goes to the CUDA library; nothing here computes on the CPU or through
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 import math
 from dataclasses import dataclass, field
 
@@ -129,32 +129,33 @@ class Fp4Tensor:
         return math.prod(self.shape[:-1])
 
 
-_FP4_BLOCK = {NVFP4: 16, MXFP4: 32}
-_here = contextlib.nullcontext()
+_FP4_SPAN = {NVFP4: 64, MXFP4: 128}   # elements of k of a scale tile
 
 
-def _fp4_row_bytes(k):
-    """vrb_fp4_row_bytes"""
-    return (k + 31) // 32 * 16
-
-
-def _fp4_scale_bytes(format, rows, k):
-    """vrb_fp4_scale_bytes"""
-    span = 4 * _FP4_BLOCK[format]
-    return (rows + 127) // 128 * ((k + span - 1) // span) * 512
+def _fp4_scale_address(scale, device):
+    if scale is None:
+        return None
+    if scale.dtype != F32 or scale.numel() != 1 or scale.device != device:
+        raise VrbError("fp4 tensor scale must be one F32 on the operand's device")
+    return scale.data_ptr()
 
 
 def _fp4_addresses(q, rows, k, device):
     """Device addresses of a packed operand's parts after a check of what they have to hold."""
-    codes, scales, scale = q.codes, q.scales, q.tensor_scale
-    if q.format not in _FP4_BLOCK or rows <= 0 or k <= 0 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or \
-            tuple(codes.shape) != (rows, _fp4_row_bytes(k)) or scales.numel() != _fp4_scale_bytes(q.format, rows, k):
+    codes, scales, span = q.codes, q.scales, _FP4_SPAN.get(q.format)
+    if span is None or rows <= 0 or k <= 0 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or \
+            tuple(codes.shape) != (rows, (k + 31) // 32 * 16) or scales.numel() != (rows + 127) // 128 * ((k + span - 1) // span) * 512:
         raise VrbError("fp4 operand: codes or scales do not match the shape and format")
-    if scale is not None and (scale.dtype != F32 or scale.numel() != 1 or scale.device != device):
-        raise VrbError("fp4 tensor scale must be one F32 on the operand's device")
     if not codes.is_cuda:
         raise VrbError("Tensor must be device-resident")
-    return _address(codes, device), _address(scales, device), None if scale is None else scale.data_ptr()
+    return _address(codes, device), _address(scales, device), _fp4_scale_address(q.tensor_scale, device)
+
+
+@functools.lru_cache(maxsize=4096)
+def _channels_last_workspace(index, code, batch, spatial, channels, groups):
+    """vrb_group_norm_channels_last_workspace_bytes on device `index` (its SM count decides)."""
+    with torch.cuda.device(index):
+        return _lib.load().vrb_group_norm_channels_last_workspace_bytes(code, batch, spatial, channels, groups)
 
 
 class HostScalar:
@@ -646,14 +647,13 @@ class B200Backend:
         for name, t in (("weight", weight), ("bias", bias)):
             if t is not None and t.numel() != channels:
                 raise VrbError(f"group norm {name} mismatch")
-        device = x.device
-        out = _result(out, x.shape, dtype, device)
-        if x.numel() == 0:
+        device, count = x.device, x.numel()
+        out = torch.empty_like(x) if out is None else _result(out, x.shape, dtype, device)
+        if count == 0:
             return out
         code = _CODE[dtype]
-        spatial = x.numel() // (batch * channels)
-        with torch.cuda.device(device) if device.index != torch._C._cuda_getDevice() else _here:
-            need = _lib.load().vrb_group_norm_channels_last_workspace_bytes(code, batch, spatial, channels, groups)
+        spatial = count // (batch * channels)
+        need = _channels_last_workspace(device.index, code, batch, spatial, channels, groups)
         # scratch of this call alone: torch's allocator keeps it from other streams and other captured graphs
         scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         _launch("vrb_group_norm_channels_last", device, x.data_ptr(), code, _address(weight, device), 0 if weight is None else _code(weight),
@@ -678,17 +678,21 @@ class B200Backend:
         count, device = x.numel(), x.device
         if x.dim() < 1 or count == 0:
             raise VrbError("fp4_quantize: rows and k must be positive")
-        if format not in _FP4_BLOCK:
+        span = _FP4_SPAN.get(format)
+        if span is None:
             raise VrbError(f"fp4_quantize: unknown 4-bit format {format}")
         shape = tuple(x.shape)
         k = shape[-1]
         rows = count // k
         if out is None:
-            out = Fp4Tensor(torch.empty((rows, _fp4_row_bytes(k)), dtype=torch.uint8, device=device),
-                            torch.empty(_fp4_scale_bytes(format, rows, k), dtype=torch.uint8, device=device), tensor_scale, format, shape)
+            codes = torch.empty((rows, (k + 31) // 32 * 16), dtype=torch.uint8, device=device)
+            scales = torch.empty((rows + 127) // 128 * ((k + span - 1) // span) * 512, dtype=torch.uint8, device=device)
+            out = Fp4Tensor(codes, scales, tensor_scale, format, shape)
+            codes, scales, scale = codes.data_ptr(), scales.data_ptr(), _fp4_scale_address(tensor_scale, device)
         elif out.format != format or out.tensor_scale is not tensor_scale or tuple(out.shape) != shape or out.codes.device != device:
             raise VrbError("output buffer does not match the result's shape, dtype or device")
-        codes, scales, scale = _fp4_addresses(out, rows, k, device)
+        else:
+            codes, scales, scale = _fp4_addresses(out, rows, k, device)
         _launch("vrb_fp4_quantize", device, format, x.data_ptr(), _CODE[dtype], scale, codes, scales, rows, k)
         return out
 
