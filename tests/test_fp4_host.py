@@ -54,13 +54,16 @@ def _status(lib, name, *args):
     ({"codes": A + 8}, -1, "16-byte aligned"),
     ({"scales": A + 4}, -1, "16-byte aligned"),
     ({"format": 1, "scale": A}, -1, "MXFP4 has no tensor scale"),
+    ({"scale": A + 2}, -1, "aligned to their elements"),
+    ({"x": A + 1}, -1, "aligned to their elements"),
+    ({"x": A + 2, "dtype": 0}, -1, "aligned to their elements"),
 ])
 def test_quantize_refusals(cuda_lib, change, code, text):
     a = {"format": 0, "x": A, "dtype": 2, "scale": None, "codes": A, "scales": A, "rows": 4, "k": 64} | change
     rc, why = _status(cuda_lib, "vrb_fp4_quantize", a["format"], a["x"], a["dtype"], a["scale"], a["codes"], a["scales"], a["rows"], a["k"], None)
     assert rc == code and text in why
-    if "x" not in change:
-        rc, why = _status(cuda_lib, "vrb_fp4_dequantize", a["format"], a["codes"], a["scales"], a["scale"], A, a["dtype"], a["rows"], a["k"], None)
+    if change.get("x", A) is not None:
+        rc, why = _status(cuda_lib, "vrb_fp4_dequantize", a["format"], a["codes"], a["scales"], a["scale"], a["x"], a["dtype"], a["rows"], a["k"], None)
         assert rc == code and text in why
 
 
@@ -80,6 +83,9 @@ def test_tensor_scale_refusals(cuda_lib):
     ({"format": 1, "ag": A}, -1, "MXFP4 has no tensor scale"), ({"format": 1, "bg": A}, -1, "MXFP4 has no tensor scale"),
     ({"act": 5}, -1, "unknown activation"), ({"act": -2}, -1, "unknown activation"),
     ({"ac": A + 8}, -1, "16-byte aligned"), ({"bs": A + 8}, -1, "16-byte aligned"),
+    ({"out": A + 1}, -1, "aligned to their elements"), ({"bias": A + 2, "bdt": 0}, -1, "aligned to their elements"),
+    ({"ag": A + 1}, -1, "aligned to their elements"), ({"bg": A + 2}, -1, "aligned to their elements"),
+    ({"m": 1 << 30, "n": 1 << 30}, -1, "at most 2^40 elements"),
 ])
 def test_linear_refusals(cuda_lib, change, code, text):
     a = {"format": 0, "ac": A, "as": A, "ag": None, "m": 4, "bc": A, "bs": A, "bg": None, "n": 8, "k": 64, "bias": None, "bdt": 0, "act": -1,
@@ -94,7 +100,9 @@ def test_linear_refusals(cuda_lib, change, code, text):
     ({"act": 5}, -1, "unknown activation"), ({"act": -2}, -1, "unknown activation"),
     ({"batch": 0}, -1, "shape/groups mismatch"), ({"spatial": 0}, -1, "shape/groups mismatch"), ({"channels": 0}, -1, "shape/groups mismatch"),
     ({"groups": 0}, -1, "shape/groups mismatch"), ({"groups": 3}, -1, "shape/groups mismatch"),
-    ({"channels": 1 << 25}, -1, "exceeds CUDA grid capacity"),
+    ({"channels": 1 << 25}, -1, "exceeds CUDA grid capacity"), ({"spatial": 1 << 40}, -1, "exceeds CUDA grid capacity"),
+    ({"x": A + 1}, -1, "aligned to their elements"), ({"out": A + 2, "dtype": 0}, -1, "aligned to their elements"),
+    ({"w": A + 2}, -1, "aligned to their elements"), ({"b": A + 1, "bdt": 2}, -1, "aligned to their elements"),
     ({"spatial": 1 << 20, "ws": None}, -4, "workspace needs"), ({"spatial": 1 << 20, "size": 16}, -4, "workspace needs"),
     ({"spatial": 1 << 20, "ws": A + 16}, -4, "workspace needs"),
 ])

@@ -24,6 +24,7 @@ int sm_count();
 inline cudaStream_t as_stream(vrb_stream s) { return static_cast<cudaStream_t>(s); }
 inline bool is_float_dtype(int dt) { return dt == VRB_F32 || dt == VRB_BF16; }
 inline size_t dtype_bytes(int dt) { return dt == VRB_F32 ? 4 : dt == VRB_BF16 ? 2 : 1; }
+inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 #define VRB_REQUIRE(cond, code, ...)      \

@@ -504,6 +504,7 @@ extern "C" int vrb_fp4_quantize(int format, const void* x, int dtype, const floa
     if (int rc = make_pack(p, format, rows, k, "fp4_quantize")) return rc;
     VRB_REQUIRE(format == VRB_NVFP4 || !tensor_scale, VRB_ERR_INVALID, "fp4_quantize: MXFP4 has no tensor scale");
     VRB_REQUIRE(aligned16(codes) && aligned16(scales), VRB_ERR_INVALID, "fp4_quantize: codes and scales must be 16-byte aligned");
+    VRB_REQUIRE(aligned_to(x, dtype_bytes(dtype)) && aligned_to(tensor_scale, 4), VRB_ERR_INVALID, "fp4_quantize: tensors must be aligned to their elements");
     // a thread to a scale word where the rows have one and at most half of its segments hold elements
     const bool serial = p.tile_row == 512 && k <= p.segments * 16 / 2;
     const int64_t units = p.padded_rows * (serial ? 1 : p.segments);
@@ -528,6 +529,7 @@ extern "C" int vrb_fp4_dequantize(int format, const void* codes, const void* sca
     if (int rc = make_pack(p, format, rows, k, "fp4_dequantize")) return rc;
     VRB_REQUIRE(format == VRB_NVFP4 || !tensor_scale, VRB_ERR_INVALID, "fp4_dequantize: MXFP4 has no tensor scale");
     VRB_REQUIRE(aligned16(codes) && aligned16(scales), VRB_ERR_INVALID, "fp4_dequantize: codes and scales must be 16-byte aligned");
+    VRB_REQUIRE(aligned_to(out, dtype_bytes(out_dtype)) && aligned_to(tensor_scale, 4), VRB_ERR_INVALID, "fp4_dequantize: tensors must be aligned to their elements");
     const int64_t units = rows * ((k + 15) / 16 + 1);
     const dim3 grid(static_cast<unsigned>(grid_for((units + kThreads - 1) / kThreads, 8)));
     const bool vec = aligned16(out) && k % 16 == 0;

@@ -454,13 +454,16 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
 // ------------------------------------------------------------------------------------ split kernel --
 constexpr int kSplitThreads = 192;
 constexpr int kSplitRing = 6;
-constexpr int kSplitColumns = 512;         // tensor memory: 128 accumulator columns, then 32 scale columns a buffer
 constexpr int kMostSplits = 8;             // portable cluster size
-constexpr size_t kSplitMostShared = kSplitRing * (2 * kCodeBytes + 2 * kScaleBytes) + 1024;
+constexpr size_t kSharedPerSm = 228 * 1024, kSharedPerCta = 1024;   // 1 KB of each CTA's is the system's
+constexpr int kTensorColumns = 512;        // of an SM
+constexpr int kSplitMostColumns = 256;     // of them for a CTA of the split kernel
+constexpr size_t kSplitMostShared = kSplitRing * (kCodeBytes + 2 * kScaleBytes + 64 * kStageBytes) + 1024;   // six buffers of 64 columns; four of 128 take less
 
 struct SplitArgs {
     LinearArgs linear;
     int columns;               // rows of a of a tile: 16, 32, 64 or 128
+    int tensor_columns;        // tensor memory: the accumulator's columns (32 at least), then 32 scale columns a buffer; a power of two
     int ring;                  // buffers
     int splits;                // CTAs along k: the cluster
     int stages;                // of all of k
@@ -496,7 +499,7 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
         mbarrier_init_fence();
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(&control.tensor_base)), "r"(kSplitColumns) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(&control.tensor_base)), "r"(q.tensor_columns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     fence_before();
@@ -529,6 +532,7 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
         }
     } else if (warp == 1) {
         const uint32_t instruction = instruction_descriptor<FORMAT>(kRows, q.columns);
+        const uint32_t scales_base = base + max(q.columns, 32);
         const uint32_t a_column = static_cast<uint32_t>(a0 % 128) / 32;   // where the tile's scales begin within the 128-row scale tile
         int slot = 0;
         unsigned phase = 0;
@@ -537,7 +541,7 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
             if (!wait_barrier(&control.full[slot], phase, &control.abort)) break;
             fence_after();
             const unsigned buffer = buffers + slot * buffer_bytes;
-            const uint32_t sb = base + 128 + slot * 32, sa = sb + 16;
+            const uint32_t sb = scales_base + slot * 32, sa = sb + 16;
             const uint64_t b_codes = kCodeDescriptor | ((buffer & 0x3ffffu) >> 4), a_codes = b_codes + ((kCodeBytes + 2 * kScaleBytes) >> 4);
             const uint64_t scales = kScaleDescriptor | (((buffer + kCodeBytes) & 0x3ffffu) >> 4);
             const int64_t left = p.k - static_cast<int64_t>(stage) * kStageElements;
@@ -631,7 +635,7 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
         for (int i = 0; i < 100000 && now_ns() - start < 20000000ull; ++i) __nanosleep(1000);
     }
     fence_after();
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(kSplitColumns));
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(q.tensor_columns));
 }
 
 // ----------------------------------------------------------------------------------------- host side --
@@ -755,12 +759,24 @@ int launch_split(const LinearMaps& maps, const LinearArgs& p, const LinearPlan& 
     q.stages = static_cast<int>((p.k + kStageElements - 1) / kStageElements);
     q.a_tiles = static_cast<unsigned>((p.m + q.columns - 1) / q.columns);
     const int own = (q.stages + q.splits - 1) / q.splits;
+    const int accumulator = q.columns < 32 ? 32 : q.columns, most = (kSplitMostColumns - accumulator) / 32;   // three buffers do as well as six, given time
     q.ring = own < kSplitRing ? own : kSplitRing;
+    if (q.ring > most) q.ring = most;
     const size_t buffer = kCodeBytes + 2 * kScaleBytes + ((static_cast<size_t>(q.columns) * kStageBytes + 1023) & ~size_t{1023});
     size_t bytes = q.ring * buffer;
     if (bytes < static_cast<size_t>(q.columns) * 512) bytes = static_cast<size_t>(q.columns) * 512;
     bytes += 1024;
+    // A CTA takes at least the share of an SM's shared memory that it takes of the tensor memory (as the pair kernel does, with
+    // all of both).  So whatever CTAs of these kernels share an SM, from one launch or several streams, no tensor memory
+    // allocation ever waits: two clusters that waited for each other's CTAs would wait for good.
+    q.tensor_columns = 32;
+    while (q.tensor_columns < accumulator + 32 * q.ring) q.tensor_columns *= 2;
+    const size_t share = kSharedPerSm * q.tensor_columns / kTensorColumns;
+    if (bytes + kSharedPerCta < share) bytes = share - kSharedPerCta;
     static_assert(kSplitMostShared + sizeof(SplitControl) <= 227 * 1024, "ring does not fit shared memory");
+    static_assert(kSplitMostShared + kSharedPerCta >= kSharedPerSm * kSplitMostColumns / kTensorColumns &&
+                      kSplitMostShared >= (kSplitMostColumns - 128) / 32 * (2 * kCodeBytes + 2 * kScaleBytes) + 1024,
+                  "the most shared memory covers the most tensor memory and the widest tile");
     static std::atomic<uint64_t> allowed{0};
     if (int rc = allow_shared(fp4_linear_split_kernel<FORMAT, ACT>, kSplitMostShared, allowed)) return rc;
     const int64_t tiles = ((p.m + q.columns - 1) / q.columns) * ((p.n + kRows - 1) / kRows);
@@ -818,6 +834,9 @@ extern "C" int vrb_fp4_linear(int format, const void* a_codes, const void* a_sca
     VRB_REQUIRE(activation >= VRB_NO_ACTIVATION && activation <= VRB_RELU, VRB_ERR_INVALID, "fp4_linear: unknown activation %d", activation);
     VRB_REQUIRE(aligned16(a_codes) && aligned16(a_scales) && aligned16(b_codes) && aligned16(b_scales), VRB_ERR_INVALID,
                 "fp4_linear: codes and scales must be 16-byte aligned");
+    VRB_REQUIRE(aligned_to(out, dtype_bytes(out_dtype)) && (!bias || aligned_to(bias, dtype_bytes(bias_dtype))) && aligned_to(a_tensor_scale, 4) &&
+                    aligned_to(b_tensor_scale, 4),
+                VRB_ERR_INVALID, "fp4_linear: tensors must be aligned to their elements");
     LinearArgs p{};
     p.a_scale = a_tensor_scale; p.b_scale = b_tensor_scale;
     p.bias = bias; p.bias_dt = bias_dtype; p.out = out; p.out_dt = out_dtype; p.activation = activation;

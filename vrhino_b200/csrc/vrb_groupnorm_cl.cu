@@ -490,7 +490,7 @@ bool one_group(const GclGeom& g, int v) { return g.groups == 1 || (g.row % v == 
 int make_geom(GclGeom& g, int64_t batch, int64_t spatial, int64_t channels, int groups) {
     VRB_REQUIRE(batch > 0 && spatial > 0 && channels > 0 && groups > 0 && channels % groups == 0, VRB_ERR_INVALID,
                 "group_norm_channels_last: group norm shape/groups mismatch");
-    VRB_REQUIRE(channels <= (int64_t{1} << 24) && batch <= (int64_t{1} << 20), VRB_ERR_INVALID,
+    VRB_REQUIRE(channels <= (int64_t{1} << 24) && batch <= (int64_t{1} << 20) && spatial <= (int64_t{1} << 40) / channels / batch, VRB_ERR_INVALID,
                 "group_norm_channels_last: group norm launch extent exceeds CUDA grid capacity");
     g.batch = batch; g.spatial = spatial; g.entry = spatial * channels;
     g.channels = g.row = static_cast<int>(channels); g.fold = 1; g.tail = 0; g.groups = groups; g.per = static_cast<int>(channels / groups);
@@ -651,6 +651,9 @@ extern "C" int vrb_group_norm_channels_last(const void* x, int dtype, const void
     VRB_REQUIRE(is_float_dtype(dtype), VRB_ERR_UNSUPPORTED, "group_norm_channels_last: dtype must be F32 or BF16");
     VRB_REQUIRE((!weight || is_float_dtype(weight_dtype)) && (!bias || is_float_dtype(bias_dtype)), VRB_ERR_UNSUPPORTED,
                 "group_norm_channels_last: weight and bias must be F32 or BF16");
+    VRB_REQUIRE(aligned_to(x, dtype_bytes(dtype)) && aligned_to(out, dtype_bytes(dtype)) && (!weight || aligned_to(weight, dtype_bytes(weight_dtype))) &&
+                    (!bias || aligned_to(bias, dtype_bytes(bias_dtype))),
+                VRB_ERR_INVALID, "group_norm_channels_last: tensors must be aligned to their elements");
     VRB_REQUIRE(activation >= VRB_NO_ACTIVATION && activation <= VRB_RELU, VRB_ERR_INVALID,
                 "group_norm_channels_last: unknown activation %d", activation);
     GclGeom g;
