@@ -39,12 +39,15 @@ def _check_pack(q, x, fmt, g=None):
 # ------------------------------------------------------------------------------------------- packing --
 @pytest.mark.parametrize("fmt", [0, 1])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("rows,k", [(1, 1), (1, 16), (2, 15), (3, 33), (5, 31), (128, 64), (129, 65), (37, 1000), (257, 999), (31, 1536), (2, 8200)])
+@pytest.mark.parametrize("rows,k", [(1, 1), (1, 16), (2, 15), (3, 33), (5, 31), (128, 64), (129, 65), (37, 1000), (257, 999), (31, 1536), (2, 8200),
+                                    (300, 5), (200, 17), (130, 48), (400, 63)])
 def test_pack_is_exact(gpu, fmt, dtype, rows, k):
     be, ops = gpu
-    x = _data(rows, k, _dtype(dtype), rows * 7 + k, 3.0)
-    g = be.fp4_tensor_scale(x) if fmt == ops.NVFP4 else None
-    _check_pack(be.fp4_quantize(x, fmt, g), x, fmt, g)
+    buffer = _data(1, rows * k + 3, _dtype(dtype), rows * 7 + k, 3.0)[0]
+    for shift in (0, 1, 3):   # on and off a 16-byte boundary
+        x = buffer[shift:shift + rows * k].view(rows, k)
+        g = be.fp4_tensor_scale(x) if fmt == ops.NVFP4 else None
+        _check_pack(be.fp4_quantize(x, fmt, g), x, fmt, g)
 
 
 @pytest.mark.parametrize("g", [1.0, 0.37, 3.0e-5, 1.1e20, 2.0 ** -110, 3.0e38, 1.0e-42])
@@ -122,7 +125,7 @@ def test_tensor_scale(gpu):
 
 @pytest.mark.parametrize("fmt", [0, 1])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("rows,k", [(1, 1), (3, 33), (129, 64), (200, 999), (7, 1536)])
+@pytest.mark.parametrize("rows,k", [(1, 1), (3, 33), (129, 64), (200, 999), (7, 1536), (77, 5), (1001, 17), (300, 63), (40, 65), (9, 2051)])
 def test_unpack_is_exact(gpu, fmt, dtype, rows, k):
     """All codes and scale bytes at random (NaN scales among them)."""
     import torch
@@ -136,9 +139,12 @@ def test_unpack_is_exact(gpu, fmt, dtype, rows, k):
     with np.errstate(over="ignore", invalid="ignore"):
         want = (e * s).astype(np.float32) * (g if g is not None else np.float32(1.0))
     want = torch.from_numpy(want).to(_dtype(dtype))
-    got = be.fp4_dequantize(q, _dtype(dtype)).cpu()
-    assert torch.equal(torch.isnan(got), torch.isnan(want))
-    assert torch.equal(torch.nan_to_num(got, 0.0), torch.nan_to_num(want, 0.0))
+    for shift in (0, 1, 3):   # the result on and off a 16-byte boundary, and what lies around it
+        buffer = torch.full((rows * k + 16,), 7.0, device="cuda", dtype=_dtype(dtype))
+        got = be.fp4_dequantize(q, _dtype(dtype), out=buffer[shift:shift + rows * k].view(rows, k)).cpu()
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(torch.nan_to_num(got, 0.0), torch.nan_to_num(want, 0.0))
+        assert (buffer[:shift] == 7.0).all() and (buffer[shift + rows * k:] == 7.0).all()
 
 
 def test_pack_and_unpack_past_32_bit_offsets(gpu):
