@@ -330,6 +330,55 @@ def test_captured_and_replayed(gpu, m):
                 assert torch.equal(outs[i], want[order[i]])
 
 
+def test_first_calls_of_a_process_are_captured(gpu):
+    """No call of the library before the capture: attributes, occupancy and the encoder are looked up while capturing."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from vrhino_b200 import ops
+be = ops.B200Backend()
+x = {m: torch.randn((m, 640), device="cuda").bfloat16() for m in (2, 40, 700)}
+h = {s: torch.randn((1, s, 64), device="cuda").bfloat16() for s in (50, 60000)}
+w = torch.randn((900, 640), device="cuda")
+torch.cuda.synchronize()
+def run():
+    q = be.fp4_quantize(w, 0, be.fp4_tensor_scale(w))
+    y = [be.fp4_linear(be.fp4_quantize(x[m], 0, q.tensor_scale), q) for m in x]
+    return y + [be.group_norm_channels_last(h[s], 8, None, None, 1e-6, activation=0) for s in h] + [be.fp4_dequantize(q)]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    captured = run()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(captured, run()))
+print("captured")
+"""
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=root, timeout=120)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
+
+
+def test_many_clusters_on_many_streams(gpu):
+    """Clusters along k of several shapes, more at once than the SMs hold, from eight streams: allocations of tensor memory must
+    not wait for each other."""
+    import torch
+    be, ops = gpu
+    jobs = [(_packed(be, ops, m, k, 0, m), _packed(be, ops, n, k, 0, m + 1)) for m, k, n in
+            ((1, 512, 4096), (2, 8192, 512), (16, 4096, 1024), (30, 2048, 3000), (64, 8192, 640), (100, 4096, 900), (300, 512, 300), (600, 1024, 2000))]
+    want = [be.fp4_linear(a, b) for a, b in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(30):
+        for i, (a, b) in enumerate(jobs):
+            with torch.cuda.stream(streams[i]):
+                got.append(be.fp4_linear(a, b))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i % len(jobs)]) for i, y in enumerate(got))
+
+
 def test_two_streams_at_once(gpu):
     import torch
     be, ops = gpu
