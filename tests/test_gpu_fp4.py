@@ -79,6 +79,23 @@ def test_pack_at_rounding_borders(gpu, g):
     _check_pack(be.fp4_quantize(t, ops.NVFP4, scale), t, ref.NVFP4, gf)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("g", [1.0, 0.125, 1.0 / 3.0, 0.7, 3.0 / 2688.0, 1.875 / 2688.0, 1.9453125 / 2688.0, 1.7890625 / 2688.0])
+def test_pack_values_of_few_bits(gpu, dtype, g):
+    """Values of three to eight significant bits under tensor scales that put them on or within an F32 step of the borders:
+    exact ties, and blocks in which every value is next to one."""
+    import torch
+    be, ops = gpu
+    rng = np.random.default_rng(11)
+    bits = rng.integers(2, 8, (256, 1))
+    x = np.round(rng.uniform(-1, 1, (256, 256)) * 2.0 ** bits) / 2.0 ** bits * 2.0 ** rng.integers(-6, 3, (256, 1))
+    x[:, ::16] = rng.choice([1.0, 1.5, 1.75, 1.25, 1.125, 1.875], (256, 16)) * 2.0 ** rng.integers(-3, 4, (256, 16))
+    t = torch.from_numpy(x).cuda().to(_dtype(dtype))
+    scale = torch.tensor([g], device="cuda", dtype=torch.float32)
+    _check_pack(be.fp4_quantize(t, ops.NVFP4, scale), t, ref.NVFP4, np.float32(g))
+    _check_pack(be.fp4_quantize(t, ops.MXFP4), t, ref.MXFP4)
+
+
 @pytest.mark.parametrize("fmt", [0, 1])
 def test_pack_special_values(gpu, fmt):
     """Zeros, infinities, NaN, subnormals and the largest values, each in a block of its own and mixed."""

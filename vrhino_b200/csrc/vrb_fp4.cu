@@ -7,13 +7,16 @@
 //
 // Rounding is that of the real quotients a / (6 g) -> e4m3 and x / (g s) -> e2m1.  The fast form multiplies by an F32
 // quotient (its 2 ulp and three roundings: relative error < 2^-21) and converts the product moved up and down by kGuard = 2^-20:
-// where both give one code it is the right one.  Where they differ a rounding border t lies between, and eight elements are
-// done again (refined8): with s g = hi + lo in F32 (one product and one multiply-add, exact) a residual step gives the quotient
-// y to within an F32 step, so y is on t's right side unless it is t itself; then |x| - t hi is exact and a multiply-add with
-// -t lo rounds to the right sign, which moves y off the border; 0 is the tie.  bf16 data meets the borders of NVFP4 to within
-// 2^-24 all the time (the tensor scale is amax / (2^7 3 7), whose factors the scales 9, 12, 14 and 15 eighths share), and more
-// or less of it with amax, so the second form has no loop over elements: 13824 x 5120 bf16 took 99 us with a search in double
-// and 36 to 78, by amax, with a loop over the elements concerned.
+// where both give one code it is the right one.  Where they differ a rounding border t lies between.  With s g = hi + lo in F32
+// (one product and one multiply-add, exact) |x| - t hi is exact next to the border and a multiply-add with -t lo rounds to the
+// sign that decides; 0 is the tie.
+//   bf16: one element decides for its block.  Elements next to borders have x / t within 2^-19 of s g, and two such quotients of
+//   8-bit by 3-bit significands are equal or 2^-11 apart; so all of them are on the same side, and the block takes the codes of
+//   the product moved up, or down, or, on a tie, the form below.  (bf16 data meets the borders of NVFP4 to within 2^-24 all the
+//   time: the tensor scale is amax / (2^7 3 7), whose factors the scales 9, 12, 14 and 15 eighths share.)
+//   F32: the eight elements are done again (refined8): a residual step gives the quotient y to within an F32 step, so y is on t's
+//   right side unless it is t itself; then the sign above moves it off the border.
+// 13824 x 5120 bf16 took 99 us with a search in double, and 51 to 76, by amax, with refined8 for both types.
 #include "vrb_fp4.cuh"
 
 namespace vrb {
@@ -57,6 +60,10 @@ __device__ __noinline__ uint32_t nv_scale_exact(float a, float g) {
         if (q < border || (q == border && (c & 1u) == 0u)) return c;
     }
     return code < 126u ? code + 1u : 126u;
+}
+// the border above the magnitude of an e2m1 code: .25 .75 1.25 1.75 2.5 3.5 5, in quarters a byte each
+__device__ __forceinline__ float e2m1_border(uint32_t magnitude) {
+    return 0.25f * static_cast<float>(__byte_perm(0x07050301u, 0x00140e0au, magnitude) & 0xffu);
 }
 // one element in double, for tensor scales outside the range of the F32 form
 __device__ __noinline__ uint32_t e2m1_exact(float x, double unit) {
@@ -266,22 +273,40 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const T* __restr
                 if (byte != 0u && byte != 0x7fu) {
                     const float s = e4m3_value(byte), hi = __fmul_rn(s, g), lo = __fmaf_rn(s, g, -hi);
                     const float r = __fdividef(1.0f, hi);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float y[8];
-                        scale8(v + h * 8, r * (1.0f - kGuard), y);
-                        uint32_t w = e2m1x8(y);
-                        scale8(v + h * 8, r * (1.0f + kGuard), y);
-                        const uint32_t above = e2m1x8(y);
-                        if (!fast) {
-                            w = 0u;
+                    float y[8];
+                    scale8(v, r * (1.0f - kGuard), y);
+                    word0 = e2m1x8(y);
+                    scale8(v + 8, r * (1.0f - kGuard), y);
+                    word1 = e2m1x8(y);
+                    scale8(v, r * (1.0f + kGuard), y);
+                    const uint32_t above0 = e2m1x8(y);
+                    scale8(v + 8, r * (1.0f + kGuard), y);
+                    const uint32_t above1 = e2m1x8(y);
+                    if (!fast) {
+                        const double step = static_cast<double>(s) * static_cast<double>(g);
+                        word0 = word1 = 0u;
 #pragma unroll 1
-                            for (int i = 0; i < 8; ++i) w |= e2m1_exact(pick8(v + h * 8, i), static_cast<double>(s) * static_cast<double>(g)) << (4 * i);
-                        } else if (w != above) {
-                            refined8(v + h * 8, hi, lo, r, y);
-                            w = e2m1x8(y);
+                        for (int i = 0; i < 8; ++i) {
+                            word0 |= e2m1_exact(pick8(v, i), step) << (4 * i);
+                            word1 |= e2m1_exact(pick8(v + 8, i), step) << (4 * i);
                         }
-                        (h ? word1 : word0) = w;
+                    } else if (word0 != above0 || word1 != above1) {
+                        bool refine = true;
+                        if constexpr (sizeof(T) == 2) {
+                            const bool first = word0 != above0;
+                            const uint32_t below = first ? word0 : word1;
+                            const int i = (__ffs(static_cast<int>(below ^ (first ? above0 : above1))) - 1) >> 2;
+                            const float a = fabsf(first ? pick8(v, i) : pick8(v + 8, i)), t = e2m1_border(below >> (4 * i) & 7u);
+                            const float d = __fmaf_rn(-t, lo, __fmaf_rn(-t, hi, a));
+                            if (d > 0.0f) { word0 = above0; word1 = above1; }
+                            refine = d == 0.0f;
+                        }
+                        if (refine) {
+                            refined8(v, hi, lo, r, y);
+                            word0 = e2m1x8(y);
+                            refined8(v + 8, hi, lo, r, y);
+                            word1 = e2m1x8(y);
+                        }
                     }
                 }
             } else {
