@@ -206,7 +206,7 @@ struct PackGeom {
 // LANES threads share a word of the scale tile (a segment of 16 elements each); 1: a thread takes all of a word's segments in
 // turn, for rows so short that most segments of a word are padding.
 template <typename T, int FORMAT, bool VEC, int LANES>
-__global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const T* __restrict__ x, const float* tensor_scale, uint8_t* __restrict__ codes,
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) fp4_quantize_kernel(const T* __restrict__ x, const float* tensor_scale, uint8_t* __restrict__ codes,
                                                                uint8_t* __restrict__ scales, PackGeom p) {
     constexpr int kPerWord = FORMAT == VRB_NVFP4 ? 4 : 8;      // segments of a scale word
     constexpr int kSerial = LANES == 1 ? kPerWord : 1;
@@ -216,14 +216,14 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const T* __restr
     const bool fast = g >= 7.888609052210118e-31f && g <= 1.2676506002282294e30f;
     const float g6 = __fmul_rn(6.0f, g);
     const int64_t units = p.segments / kSerial;                // of a row
-    const int64_t total = p.padded_rows * units, stride = static_cast<int64_t>(gridDim.x) * kThreads;
+    const int64_t total = p.rows * units, stride = static_cast<int64_t>(gridDim.x) * kThreads;
     int64_t u = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
     const int64_t d_row = stride / units, d_unit = stride - d_row * units;
     int64_t row = u / units, unit = u - row * units;
     const int lane = threadIdx.x & 31;
     const int64_t count = p.rows * p.k;
     auto fetch = [&](int64_t r, int64_t column, uint32_t (&w)[Elements<T>::kWords]) {
-        if (r < p.rows && column < p.k) load16<T, VEC>(x, count, x + r * p.k + column, column, p.k, w);
+        if (column < p.k) load16<T, VEC>(x, count, x + r * p.k + column, column, p.k, w);
         else
 #pragma unroll
             for (int i = 0; i < Elements<T>::kWords; ++i) w[i] = 0u;
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const T* __restr
         if (next_unit >= units) { next_unit -= units; ++next_row; }
         uint32_t word = 0u, carried = 0u;
         // a short row's segments past its codes have nothing to write but the zero scales that `carried` begins with
-        const int parts = LANES > 1 ? 1 : row >= p.rows ? 0 : static_cast<int>(p.row_bytes / 8 < kSerial ? p.row_bytes / 8 : kSerial);
+        const int parts = LANES > 1 ? 1 : static_cast<int>(p.row_bytes / 8 < kSerial ? p.row_bytes / 8 : kSerial);
 #pragma unroll 1
         for (int part = 0; part < parts; ++part) {
             const int64_t segment = unit * kSerial + part, column = segment * 16;
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const T* __restr
                 fetch(row, column, w);
                 top = values16<T>(w, v);
             }
-            const bool live = row < p.rows && column < p.k;
+            const bool live = column < p.k;
             uint32_t byte = 0u, word0 = 0u, word1 = 0u;
             if constexpr (FORMAT == VRB_NVFP4) {
                 const float a = __uint_as_float(top);
@@ -332,10 +332,10 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const T* __restr
                     word1 = e2m1x8(y);
                 }
             }
-            if (row < p.rows && segment * 8 < p.row_bytes)
+            if (segment * 8 < p.row_bytes)
                 *reinterpret_cast<uint2*>(codes + row * p.row_bytes + segment * 8) = make_uint2(word0, word1);
             constexpr int kPerBlock = FORMAT == VRB_NVFP4 ? 1 : 2;   // segments of a block
-            const bool in_block = row < p.rows && (FORMAT == VRB_NVFP4 ? column < p.k : (segment & ~int64_t{1}) * 16 < p.k);
+            const bool in_block = FORMAT == VRB_NVFP4 ? column < p.k : (segment & ~int64_t{1}) * 16 < p.k;
             word = in_block ? byte : 0u;
             if constexpr (LANES > 1) {
                 word |= __shfl_xor_sync(group, word, kPerBlock) << 8;
@@ -351,6 +351,12 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const T* __restr
         }
         row = next_row;
         unit = next_unit;
+    }
+    // the scales of the rows that fill the last tile up
+    const int64_t words = p.tile_row / 512, filling = (p.padded_rows - p.rows) * words;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < filling; i += stride) {
+        const int64_t r = p.rows + i / words;
+        *reinterpret_cast<uint32_t*>(scales + (r >> 7) * p.tile_row + i % words * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4) = 0u;
     }
 }
 
@@ -573,8 +579,8 @@ extern "C" int vrb_fp4_quantize(int format, const void* x, int dtype, const floa
     VRB_REQUIRE(aligned_to(x, dtype_bytes(dtype)) && aligned_to(tensor_scale, 4), VRB_ERR_INVALID, "fp4_quantize: tensors must be aligned to their elements");
     // a thread to a scale word where the rows have one and at most half of its segments hold elements
     const bool serial = p.tile_row == 512 && k <= p.segments * 16 / 2;
-    const int64_t units = p.padded_rows * (serial ? 1 : p.segments);
-    const dim3 grid(static_cast<unsigned>(grid_for((units + kThreads - 1) / kThreads, 8)));
+    const int64_t units = rows * (serial ? 1 : p.segments), filling = (p.padded_rows - rows) * (p.tile_row / 512);
+    const dim3 grid(static_cast<unsigned>(grid_for((units + filling + kThreads - 1) / kThreads, 8)));
     const bool vec = aligned16(x) && k % (16 / static_cast<int64_t>(dtype_bytes(dtype))) == 0;
     cudaStream_t s = as_stream(stream);
 #define VRB_PACK(T, F, V, L) launch_overlapped(fp4_quantize_kernel<T, F, V, L>, grid, dim3(kThreads), 0, s, static_cast<const T*>(x), tensor_scale, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), p)
