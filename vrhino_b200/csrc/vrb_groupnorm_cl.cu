@@ -153,38 +153,21 @@ struct Sums {
 // group's {S, Q} goes to `take(group - first group of the slab, S, Q)` on lane 0.
 template <int THREADS, int D, int V, typename Take>
 __device__ __forceinline__ void add_groups(double (&sums)[2][THREADS * D], const GclGeom& g, int slab0, int slab, Take take) {
-    const int lane = threadIdx.x & 31, c_begin = slab0 * V, c_end = c_begin + slab * V, first = c_begin / g.per;
     constexpr int E = V / D;   // channels of an entry
-    if (g.fold > 1) {          // one slab; a group's channels come `fold` times
-        const int width = g.per * (g.groups == 1 ? g.fold : 1) / E, times = g.groups == 1 ? 1 : g.fold;
-        for (int group = threadIdx.x >> 5; group < g.groups; group += THREADS / 32) {
-            double s = 0.0, q = 0.0;
-            for (int i = lane; i < g.rpp * times * width; i += 32) {
-                const int r = i / (times * width), j = (i - r * times * width) / width, at = i - (r * times + j) * width;
-                const int k = r * g.slab * D + (j * g.row + group * g.per) / E + at;
-                s += sums[0][k];
-                q += sums[1][k];
-            }
-            for (int offset = 16; offset > 0; offset >>= 1) {
-                s += __shfl_xor_sync(0xffffffffu, s, offset);
-                q += __shfl_xor_sync(0xffffffffu, q, offset);
-            }
-            if (lane == 0) take(group, s, q);
-        }
-        return;
-    }
-    for (int group = first + (threadIdx.x >> 5); group * g.per < c_end; group += THREADS / 32) {
-        const int from = (max(group * g.per, c_begin) - c_begin) / E, width = (min((group + 1) * g.per, c_end) - c_begin) / E - from;
+    const int lane = threadIdx.x & 31, c_begin = slab0 * V, c_end = c_begin + slab * V, first = c_begin / g.per;
+    // a folded row (one slab) holds a group's channels `times` times, the only group's one after the other
+    const int times = g.groups == 1 ? 1 : g.fold, span = g.groups == 1 ? g.channels : g.per;
+    for (int group = first + (threadIdx.x >> 5); group < g.groups && group * span < c_end; group += THREADS / 32) {
+        const int from = (max(group * span, c_begin) - c_begin) / E, width = (min((group + 1) * span, c_end) - c_begin) / E - from;
         double s = 0.0, q = 0.0;
-        int r = 0, at = lane;
-        while (at >= width && r < g.rpp) { at -= width; ++r; }
-        while (r < g.rpp) {
-            const int i = r * g.slab * D + from + at;
-            s += sums[0][i];
-            q += sums[1][i];
-            at += 32;
-            while (at >= width && r < g.rpp) { at -= width; ++r; }
+#pragma unroll 1
+        for (int i = lane; i < g.rpp * times * width; i += 32) {
+            const int rt = i / width, r = times > 1 ? rt / times : rt;
+            const int k = r * g.slab * D + (rt - r * times) * g.row / E + from + (i - rt * width);
+            s += sums[0][k];
+            q += sums[1][k];
         }
+#pragma unroll 1
         for (int offset = 16; offset > 0; offset >>= 1) {
             s += __shfl_xor_sync(0xffffffffu, s, offset);
             q += __shfl_xor_sync(0xffffffffu, q, offset);
@@ -282,21 +265,33 @@ __device__ __forceinline__ void collect_groups(const double* partial, int64_t b,
     double2 sum = make_double2(0.0, 0.0);
     if (share < shares) {
         const double2* p = reinterpret_cast<const double2*>(partial) + b * g.splits * g.groups + first + group;
-#pragma unroll 8
-        for (int i = share; i < g.splits; i += shares) {
-            const double2 v = p[static_cast<int64_t>(i) * g.groups];
-            sum.x += v.x;
-            sum.y += v.y;
+        constexpr int U = 8;   // loads in flight: one after the other, each waits for L2
+        for (int i = share; i < g.splits; i += U * shares) {
+            double2 v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = i + u * shares < g.splits ? p[static_cast<int64_t>(i + u * shares) * g.groups] : make_double2(0.0, 0.0);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                sum.x += v[u].x;
+                sum.y += v[u].y;
+            }
         }
     }
     parts[threadIdx.x] = sum;
     __syncthreads();
-    if (threadIdx.x < count) {
-        for (int i = 1; i < shares; ++i) {
-            sum.x += parts[i * count + group].x;
-            sum.y += parts[i * count + group].y;
+    for (int group = threadIdx.x >> 5; group < count; group += THREADS / 32) {
+        sum = make_double2(0.0, 0.0);
+        for (int i = threadIdx.x & 31; i < shares; i += 32) {
+            const double2 v = parts[i * count + group];
+            sum.x += v.x;
+            sum.y += v.y;
         }
-        take(group, moments_to_stats(sum.x, sum.y, g.share, eps));
+#pragma unroll 1
+        for (int offset = 16; offset > 0; offset >>= 1) {
+            sum.x += __shfl_xor_sync(0xffffffffu, sum.x, offset);
+            sum.y += __shfl_xor_sync(0xffffffffu, sum.y, offset);
+        }
+        if ((threadIdx.x & 31) == 0) take(group, moments_to_stats(sum.x, sum.y, g.share, eps));
     }
     __syncthreads();
 }
@@ -321,7 +316,21 @@ __device__ __forceinline__ void load_channels(const void* p, int dt, int c0, int
         return;
     }
     int c = c0;
-    if (dt == VRB_F32) {
+    // one or two wide loads where they lie whole and aligned: V loads of 2 bytes cost a CTA of 1024 threads 3 us
+    if (V >= 4 && c0 + V <= channels && (reinterpret_cast<uintptr_t>(p) + (dt == VRB_F32 ? 4 : 2) * static_cast<uintptr_t>(c0)) % (dt == VRB_F32 ? 16 : 2 * V) == 0) {
+        if (dt == VRB_F32) {
+#pragma unroll
+            for (int e = 0; e < V; e += 4) {
+                const Vec<float, 4> w = load_vec<false, float, 4>(static_cast<const float*>(p) + c0 + e);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[(e + i) % V] = w.get(i);
+            }
+        } else {
+            const Vec<uint16_t, V> w = load_vec<false, uint16_t, V>(static_cast<const uint16_t*>(p) + c0);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = w.get(e);
+        }
+    } else if (dt == VRB_F32) {
 #pragma unroll
         for (int e = 0; e < V; ++e) { v[e] = static_cast<const float*>(p)[c]; if (++c == channels) c = 0; }
     } else {
