@@ -6,7 +6,7 @@
 //
 // Pair kernel: persistent pairs of CTAs (two SMs of a TPC) on 256 x 256 output tiles.  Each CTA holds 128 rows of a and
 // 128 of b; the products read both halves, so a byte brought to an SM takes part in twice the products of a
-// 128 x 128 tile, which L2 bandwidth asks for.  Ten warps:
+// 128 x 128 tile, which L2 bandwidth asks for.  Eighteen warps:
 //   warp 0      copies 256 elements of k at a time into a ring of buffers: codes by tensor map (128-byte swizzle,
 //               zeros outside the operand), scale tiles by a map of 8-byte words
 //   warp 1      of the pair's first CTA copies the scale tiles on into tensor memory and issues the products; a
