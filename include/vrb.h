@@ -1,5 +1,6 @@
 /*
- * vrb.h -- C ABI of the B200 (sm_100a) non-GEMM operator library for the vrhino runtime.
+ * vrb.h -- C ABI of the B200 (sm_100a) operator library for the vrhino runtime: the non-GEMM operators,
+ * and microscaled 4-bit packing with the linear that takes packed operands.
  *
  * This is the boundary a vrhino::Backend implementation binds to: every entry point takes
  * raw DEVICE pointers, sizes and a CUDA stream, allocates nothing, never synchronises, launches
