@@ -91,18 +91,24 @@ __device__ __forceinline__ void store_vec(float* p, const float (&v)[V]) {
     else __stcs(p, v[0]);
 }
 
-// The activation on an F32 value that is rounded once afterwards.  SiLU and GELU-tanh go through one exponential and
-// one reciprocal (x sigmoid(x); x sigmoid(2u), u the tanh form's argument): relative error below 2^-20 where the result
-// is not negligible, far under the bf16 step and the F32 statistics' own error.  ACT 3: any other kind.
-template <int ACT>
-__device__ __forceinline__ float activate(float y, int kind) {
-    if constexpr (ACT == 0) return y;
-    if constexpr (ACT == 1) return __fdividef(y, 1.0f + __expf(-y));
-    if constexpr (ACT == 2) {
-        const float u = 0.7978845608028654f * (y + 0.044715f * y * y * y);
-        return __fdividef(y, 1.0f + __expf(-2.0f * u));
+// act((v - mean) scale + shift) of a thread's V channels: F32 values that are rounded once afterwards.  SiLU and GELU-tanh by
+// pairs (gate_pair: three special functions for two values; with four the normalise pass of 25 MB waits for that unit).  ACT 3:
+// any other kind.
+template <int ACT, typename T, int V>
+__device__ __forceinline__ void normalise(const Vec<T, V>& v, const float (&mean)[V], const float (&scale)[V], const float (&shift)[V], int kind, float (&y)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) y[e] = fmaf(v.get(e) - mean[e], scale[e], shift[e]);
+    if constexpr (ACT == 1 || ACT == 2) {
+#pragma unroll
+        for (int e = 0; e + 1 < V; e += 2) gate_pair<ACT>(pack_f32x2(y[e], y[e + 1]), y[e], y[e + 1]);
+        if constexpr (V == 1) {
+            float unused;
+            gate_pair<ACT>(pack_f32x2(y[0], 0.0f), y[0], unused);
+        }
+    } else if constexpr (ACT == 3) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) y[e] = activation_value(kind, y[e]);
     }
-    return activation_value(kind, y);
 }
 
 // Sums of a thread's V channels over a run, and what has been rebuilt from earlier runs.  WHOLE: the V channels lie in one group
@@ -391,8 +397,7 @@ __global__ void __launch_bounds__(kApplyThreads, 1) gcl_apply_kernel(const T* x,
         for (int u = 0; u < U; ++u)
             if (row - u * step >= 0) {
                 float y[V];
-#pragma unroll
-                for (int e = 0; e < V; ++e) y[e] = activate<ACT>(fmaf(v[u].get(e) - mean[e], scale[e], shift[e]), kind);
+                normalise<ACT>(v[u], mean, scale, shift, kind, y);
                 store_vec<V>(out + at - u * p_step, y);
             }
     }
@@ -401,7 +406,13 @@ __global__ void __launch_bounds__(kApplyThreads, 1) gcl_apply_kernel(const T* x,
         const int64_t rest = b * g.entry + g.spatial * g.channels + c0;
 #pragma unroll
         for (int e = 0; e < V; ++e)
-            if (c0 + e < g.tail) store1(out, dt, rest + e, activate<ACT>(fmaf(load1(x, dt, rest + e) - mean[e], scale[e], shift[e]), kind));
+            if (c0 + e < g.tail) {
+                const Vec<T, 1> v = load_vec<true, T, 1>(x + rest + e);
+                const float m[1] = {mean[e]}, f[1] = {scale[e]}, o[1] = {shift[e]};
+                float y[1];
+                normalise<ACT>(v, m, f, o, kind, y);
+                store1(out, dt, rest + e, y[0]);
+            }
     }
 }
 
@@ -471,8 +482,7 @@ __global__ void __launch_bounds__(kClusterThreads) gcl_cluster_kernel(const T* x
         for (int i = 0; i < R; ++i)
             if (row0 + i * step < spatial) {
                 float y[V];
-#pragma unroll
-                for (int e = 0; e < V; ++e) y[e] = activate<ACT>(fmaf(v[i].get(e) - mean[e], scale[e], shift[e]), kind);
+                normalise<ACT>(v[i], mean, scale, shift, kind, y);
                 store_vec<V>(out + at0 + i * p_step, y);
             }
     }
