@@ -3,7 +3,13 @@
 Bound.  With z = (x - mean) / std * gamma: the difference, the product with rsqrt(var) * gamma (itself two roundings) and
 the final multiply-add are half an F32 step each, the F32 mean is half a step of |mean|, and the variance comes from F32
 sums of at most 32 terms next to an anchor of the data's own size, each relative 32 * 2^-24 of a second moment that is at
-most a few times the variance: below 128 * 2^-24 |z| altogether.  Activations have slopes below 1.2 and are evaluated to
+most a few times the variance: below 128 * 2^-24 |z| altogether.  The mean comes from F32 sums too, and where x lies next to
+it nothing scales its error down: a run of n <= 32 terms d = x - K adds to within n 2^-24 sum |d| (one rounding for each
+difference, n - 1 for partial sums that are no larger than sum |d|), so the mean is off by at most 32 * 2^-24 times the mean
+|d|.  In units of the group's standard deviation mean |x - mean| <= 1, and the anchors, n_r elements weighing on one of
+them, have mean |K - mean| <= sqrt(sum n_r (K_r - mean)^2 / N) <= sqrt(32): 32 (1 + sqrt(32)) < 214 steps of gamma.  That
+term falls away for small integers, whose sums are exact (|d| <= 16, s2 <= 32 * 256 < 2^24); test_exact_sums asks for the
+bound without it.  Activations have slopes below 1.2 and are evaluated to
 2^-20 of their argument; the result is rounded once."""
 import numpy as np
 import pytest
@@ -23,7 +29,7 @@ def _make(shape, dtype, seed, affine=True, offset=0.5):
     return x.to(dtype), w, b
 
 
-def _check(got, x, groups, w, b, eps, kind):
+def _check(got, x, groups, w, b, eps, kind, exact_sums=False):
     import torch
     v = x.double().flatten(1, -2).unflatten(2, (groups, -1))
     var, mean = torch.var_mean(v, dim=(1, 3), correction=0, keepdim=True)
@@ -33,6 +39,8 @@ def _check(got, x, groups, w, b, eps, kind):
     y = z + (0.0 if b is None else b.double())
     offset = (mean * inv).expand_as(v).flatten(2).abs() * (1.0 if w is None else gamma.abs())
     bound = 2.0 ** -24 * (128 * z.abs() + 2 * offset + 2 * y.abs())
+    if not exact_sums:
+        bound = bound + 2.0 ** -24 * 214 * (1.0 if w is None else gamma.abs())
     if kind is not None:
         bound = 1.2 * bound + 2.0 ** -20 * y.abs()
     want = torch.from_numpy(ref.activation(y.cpu().numpy(), kind)).cuda()
@@ -54,6 +62,13 @@ SHAPES = [
 ]
 
 
+# maps of a few MB, which L2 keeps between the passes: full and ragged last rows, slabs of several groups and of one, several entries
+MIDDLE = [
+    ((1, 4097, 512), 32), ((1, 24960, 512), 32), ((1, 26624, 256), 16), ((1, 26625, 256), 16), ((2, 1100, 320), 32), ((1, 9216, 320), 32),
+    ((1, 1500, 2048), 16), ((1, 12000, 32), 1), ((3, 6000, 128), 8), ((1, 5001, 96), 2), ((1, 9999, 192), 6), ((2, 5300, 64), 1),
+]
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("shape,groups", SHAPES)
 def test_shapes(gpu, dtype, shape, groups):
@@ -61,6 +76,31 @@ def test_shapes(gpu, dtype, shape, groups):
     be, ops = gpu
     x, w, b = _make(shape, {"bf16": torch.bfloat16, "f32": torch.float32}[dtype], sum(shape))
     _check(be.group_norm_channels_last(x, groups, w, b, 1e-6), x, groups, w, b, 1e-6, None)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("shape,groups", SHAPES + MIDDLE)
+def test_exact_sums(gpu, dtype, shape, groups):
+    """Integers up to 8: every sum is exact, so one element missing or counted twice shows in the mean."""
+    import torch
+    be, ops = gpu
+    g = torch.Generator(device="cuda").manual_seed(sum(shape))
+    x = torch.randint(-8, 9, shape, device="cuda", generator=g).to({"bf16": torch.bfloat16, "f32": torch.float32}[dtype])
+    _, w, b = _make(shape[-1:], torch.float32, 1)
+    _check(be.group_norm_channels_last(x, groups, w, b, 1e-6), x, groups, w, b, 1e-6, None, exact_sums=True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("kind", [None, 0, 2, 4])
+@pytest.mark.parametrize("shape,groups", MIDDLE)
+def test_middle_shapes(gpu, dtype, kind, shape, groups):
+    import torch
+    be, ops = gpu
+    x, w, b = _make(shape, {"bf16": torch.bfloat16, "f32": torch.float32}[dtype], sum(shape))
+    out = be.group_norm_channels_last(x, groups, w, b, 1e-6, activation=kind)
+    _check(out, x, groups, w, b, 1e-6, kind)
+    again = be.group_norm_channels_last(x, groups, w, b, 1e-6, activation=kind, out=x)   # in place, and the same bits
+    assert again.data_ptr() == x.data_ptr() and torch.equal(again, out)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])

@@ -41,7 +41,8 @@ struct GclGeom {
     double share;                  // 1 / elements of a group
 };
 
-__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 // the double at `local` in the shared memory of the cluster's CTA `rank`
 __device__ __forceinline__ double load_cluster(const double* local, unsigned rank) {
     double v;
@@ -416,6 +417,29 @@ __global__ void __launch_bounds__(kApplyThreads, 1) gcl_apply_kernel(const T* x,
     }
 }
 
+// The statistics of a slab's groups from the sums of all CTAs of a cluster (eight at most), in `own`: eight lanes to a group, a
+// CTA's sums to each, a fixed tree.  All threads of the cluster; the CTA's own sums stay until cluster_wait().
+__device__ __forceinline__ void join_cluster(const double (*mine)[2], float2* own, int groups, const GclGeom& g, float eps) {
+    __syncwarp();
+    if (g.cluster > 1) { cluster_arrive(); cluster_wait(); } else __syncthreads();
+    for (int at = threadIdx.x; at < (groups * 8 + 31) / 32 * 32; at += kClusterThreads) {
+        const int group = at >> 3, r = at & 7;
+        double s = 0.0, q = 0.0;
+        if (group < groups && r < g.cluster) {
+            s = g.cluster > 1 ? load_cluster(&mine[group][0], r) : mine[group][0];
+            q = g.cluster > 1 ? load_cluster(&mine[group][1], r) : mine[group][1];
+        }
+#pragma unroll
+        for (int offset = 4; offset > 0; offset >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, offset);
+            q += __shfl_xor_sync(0xffffffffu, q, offset);
+        }
+        if (group < groups && r == 0) own[group] = moments_to_stats(s, q, g.share, eps);
+    }
+    __syncthreads();
+    if (g.cluster > 1) cluster_arrive();   // has read the others' sums
+}
+
 // One cluster per (batch entry, slab of whole groups): up to kMostRows rows of a thread stay in registers between the statistics
 // and the result.  Row i of a thread is (i * cluster + rank) * rpp + lane_row.
 constexpr int kMostRows = 4;
@@ -463,17 +487,7 @@ __global__ void __launch_bounds__(kClusterThreads) gcl_cluster_kernel(const T* x
     }
     __syncthreads();
     add_groups<kClusterThreads, Acc::D, V>(sums, g, slab0, slab, [&](int group, double s, double q) { mine[group][0] = s; mine[group][1] = q; });
-    if (g.cluster > 1) cluster_sync(); else __syncthreads();
-    const int groups = slab * V / g.per;
-    for (int group = threadIdx.x; group < groups; group += kClusterThreads) {
-        double s = 0.0, q = 0.0;
-        for (int r = 0; r < g.cluster; ++r) {
-            s += g.cluster > 1 ? load_cluster(&mine[group][0], r) : mine[group][0];
-            q += g.cluster > 1 ? load_cluster(&mine[group][1], r) : mine[group][1];
-        }
-        own[group] = moments_to_stats(s, q, g.share, eps);
-    }
-    __syncthreads();
+    join_cluster(mine, own, slab * V / g.per, g, eps);
     if (live) {
         const int first = slab0 * V / g.per;
         float mean[V];
@@ -486,7 +500,8 @@ __global__ void __launch_bounds__(kClusterThreads) gcl_cluster_kernel(const T* x
                 store_vec<V>(out + at0 + i * p_step, y);
             }
     }
-    if (g.cluster > 1) cluster_sync();   // no CTA's memory goes while another reads it
+    __syncwarp();
+    if (g.cluster > 1) cluster_wait();   // no CTA's memory goes while another reads it
 }
 
 int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
@@ -538,7 +553,9 @@ void set_splits(GclGeom& g) {
 // more (a row's piece of a slab should fill memory sectors), its rows have to fit kMostRows rows of a thread in up to eight
 // CTAs, and all clusters should be at work at once.  Measured against the passes (bf16 with SiLU, back to back): 64 rows of 512
 // channels 4.9 us against 8.8, 256 rows 5.7 against 9.2, 2048 rows 8.0 against 11.8; with 16 rows a thread the code of a
-// once-run kernel costs more than a second read of x (4096 rows 15.9 against 12.6).
+// once-run kernel costs more than a second read of x (4096 rows 15.9 against 12.6).  Keeping a slab's rows in the shared memory of
+// its cluster instead costs more too: pieces of 64 bytes of every row come at a quarter of the rate of whole rows (24960 rows
+// 32.2 against 20.2).
 bool set_cluster(GclGeom& g, int v, int element) {
     int groups = 1;
     while (groups < g.groups && (groups * g.per % v != 0 || groups * g.per * element < 64 || g.groups % groups != 0)) ++groups;
