@@ -324,4 +324,22 @@ __device__ __forceinline__ void gate_pair(unsigned long long y, float& out0, flo
     out1 = y1 * (r * d0);
 }
 
+// CTAs at work at once, one to an SM, for clusters of 1 to 8 (processor groups are no whole multiples of a cluster): room[cluster].
+// Asked once per device, of any kernel that may have `most_shared` bytes, more than half an SM's.
+constexpr int kMostCluster = 8;            // portable cluster size
+const int* cluster_room(const void* kernel, int threads, size_t most_shared);
+
+// Lets a kernel have `bytes` of dynamic shared memory; asked once per device (`done`: a bit for each).
+template <typename Kernel>
+int allow_shared(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done, const char* what) {
+    int device = 0;
+    const bool known = cudaGetDevice(&device) == cudaSuccess && device >= 0 && device < 64;
+    const uint64_t bit = known ? uint64_t{1} << device : 0;
+    if (done.load(std::memory_order_acquire) & bit) return VRB_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    VRB_REQUIRE(e == cudaSuccess, VRB_ERR_CUDA, "CUDA error: %s (%s)", cudaGetErrorString(e), what);
+    done.fetch_or(bit, std::memory_order_release);
+    return VRB_OK;
+}
+
 }  // namespace vrb

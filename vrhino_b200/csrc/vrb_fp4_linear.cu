@@ -433,7 +433,7 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
 // ------------------------------------------------------------------------------------ split kernel --
 constexpr int kSplitThreads = 192;
 constexpr int kSplitRing = 6;
-constexpr int kMostSplits = 8;             // portable cluster size
+constexpr int kMostSplits = kMostCluster;
 constexpr size_t kSharedPerSm = 228 * 1024, kSharedPerCta = 1024;   // 1 KB of each CTA's is the system's
 constexpr int kTensorColumns = 512;        // of an SM
 constexpr int kSplitMostColumns = 256;     // of them for a CTA of the split kernel
@@ -643,19 +643,6 @@ bool encode_scales(CUtensorMap* map, int format, const void* scales, int64_t row
                      CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-// Lets a kernel have `bytes` of dynamic shared memory; asked once per device (`done`: a bit for each).
-template <typename Kernel>
-int allow_shared(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done) {
-    int device = 0;
-    const bool known = cudaGetDevice(&device) == cudaSuccess && device >= 0 && device < 64;
-    const uint64_t bit = known ? uint64_t{1} << device : 0;
-    if (done.load(std::memory_order_acquire) & bit) return VRB_OK;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-    VRB_REQUIRE(e == cudaSuccess, VRB_ERR_CUDA, "CUDA error: %s (fp4_linear)", cudaGetErrorString(e));
-    done.fetch_or(bit, std::memory_order_release);
-    return VRB_OK;
-}
-
 struct LinearMaps {
     CUtensorMap a, b, a_scales, b_scales, out;
 };
@@ -664,7 +651,7 @@ template <int FORMAT, int ACT, int OUT>
 int launch_pair(const LinearMaps& maps, const LinearArgs& p, cudaStream_t s) {
     static_assert(sizeof(PairShared) <= 227 * 1024, "ring does not fit shared memory");
     static std::atomic<uint64_t> allowed{0};
-    if (int rc = allow_shared(fp4_linear_pair_kernel<FORMAT, ACT, OUT>, sizeof(PairShared), allowed)) return rc;
+    if (int rc = allow_shared(fp4_linear_pair_kernel<FORMAT, ACT, OUT>, sizeof(PairShared), allowed, "fp4_linear")) return rc;
     const int64_t tiles = ((p.m + kPairTile - 1) / kPairTile) * ((p.n + kPairTile - 1) / kPairTile), pairs = sm_count() / 2;
     launch_overlapped(fp4_linear_pair_kernel<FORMAT, ACT, OUT>, dim3(static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs))), dim3(kPairThreads),
                       sizeof(PairShared), s, maps.a, maps.b, maps.a_scales, maps.b_scales, maps.out, p);
@@ -678,45 +665,12 @@ struct LinearPlan {
     int columns;   // 0: pair kernel
     int splits;
 };
-// CTAs of the split kernel at work at once for clusters of 1 to 8: processor groups are not whole multiples of a cluster
-const int* split_room() {
-    static std::atomic<int> known[64][kMostSplits + 1];
-    static thread_local int room[kMostSplits + 1];
-    int device = 0;
-    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) device = 0;
-    for (int splits = 1; splits <= kMostSplits; ++splits) {
-        int n = known[device][splits].load(std::memory_order_relaxed);
-        if (n == 0) {
-            n = sm_count();
-            if (splits > 1) {
-                cudaLaunchConfig_t config = {};
-                config.gridDim = dim3(static_cast<unsigned>(n / splits * splits));
-                config.blockDim = dim3(kSplitThreads);
-                config.dynamicSmemBytes = 120 * 1024;   // one CTA to an SM
-                cudaLaunchAttribute attribute;
-                attribute.id = cudaLaunchAttributeClusterDimension;
-                attribute.val.clusterDim.x = static_cast<unsigned>(splits);
-                attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-                config.attrs = &attribute;
-                config.numAttrs = 1;
-                int clusters = 0;
-                const bool asked = cudaFuncSetAttribute(fp4_linear_split_kernel<VRB_NVFP4, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSplitMostShared) == cudaSuccess &&
-                                   cudaOccupancyMaxActiveClusters(&clusters, fp4_linear_split_kernel<VRB_NVFP4, 0>, &config) == cudaSuccess && clusters > 0;
-                if (!asked) cudaGetLastError();
-                n = asked ? clusters * splits : n * 3 / 4;
-            }
-            known[device][splits].store(n, std::memory_order_relaxed);
-        }
-        room[splits] = n;
-    }
-    return room;
-}
 LinearPlan plan_linear(int64_t m, int64_t n, int stages) {
     auto ceil_div = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     LinearPlan best{0, 1};
     const int64_t pair_tiles = ceil_div(m, kPairTile) * ceil_div(n, kPairTile), pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1;
     int64_t least = 4300 + ceil_div(pair_tiles, pairs) * (static_cast<int64_t>(stages) * 290 + 500);
-    const int* room = split_room();
+    const int* room = cluster_room(reinterpret_cast<const void*>(fp4_linear_split_kernel<VRB_NVFP4, 0>), kSplitThreads, kSplitMostShared);
     for (int columns = 16; columns <= 128; columns *= 2) {
         if (columns <= 32 && m > columns) continue;   // tiles narrower than 64 would begin inside a scale word's lanes
         const int64_t tiles = ceil_div(m, columns) * ceil_div(n, kRows);
@@ -757,7 +711,7 @@ int launch_split(const LinearMaps& maps, const LinearArgs& p, const LinearPlan& 
                       kSplitMostShared >= (kSplitMostColumns - 128) / 32 * (2 * kCodeBytes + 2 * kScaleBytes) + 1024,
                   "the most shared memory covers the most tensor memory and the widest tile");
     static std::atomic<uint64_t> allowed{0};
-    if (int rc = allow_shared(fp4_linear_split_kernel<FORMAT, ACT>, kSplitMostShared, allowed)) return rc;
+    if (int rc = allow_shared(fp4_linear_split_kernel<FORMAT, ACT>, kSplitMostShared, allowed, "fp4_linear")) return rc;
     const int64_t tiles = ((p.m + q.columns - 1) / q.columns) * ((p.n + kRows - 1) / kRows);
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(static_cast<unsigned>(tiles * q.splits));

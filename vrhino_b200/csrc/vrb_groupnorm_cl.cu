@@ -11,6 +11,7 @@
 // Q = s2 + K (2 s1 + n K); threads, CTAs and clusters are added in a fixed order.
 //   Feature maps that fit the registers of one cluster per slab of channels: gcl_cluster reads x once, keeps it, adds the sums
 //   over distributed shared memory and writes the result: one launch.
+//   Feature maps that fit the shared memory of clusters at work at once: gcl_resident does the same from there.
 //   Others: 1. gcl_partial   a CTA's sums per (batch entry, group)
 //           2. gcl_finalize  only for many groups: adds the CTAs' sums once, where adding them in every CTA of 3. would cost more
 //           3. gcl_apply     sweeps the rows backwards, so that it starts with what the statistics pass left in L2
@@ -22,6 +23,7 @@ namespace {
 constexpr int kThreads = 512;      // of the statistics pass
 constexpr int kApplyThreads = 1024;// of the normalise pass: one CTA to an SM, so that the sums are added once on each
 constexpr int kClusterThreads = 256;
+constexpr int kResidentThreads = 512;
 constexpr int kRun = 32;           // rows of a thread between two rebuilds in double
 constexpr int kClusterGroups = 128;// groups of a cluster's slab, at most
 constexpr int kInlineGroups = 64;  // groups up to which gcl_apply adds the CTAs' sums itself
@@ -419,10 +421,11 @@ __global__ void __launch_bounds__(kApplyThreads, 1) gcl_apply_kernel(const T* x,
 
 // The statistics of a slab's groups from the sums of all CTAs of a cluster (eight at most), in `own`: eight lanes to a group, a
 // CTA's sums to each, a fixed tree.  All threads of the cluster; the CTA's own sums stay until cluster_wait().
+template <int THREADS>
 __device__ __forceinline__ void join_cluster(const double (*mine)[2], float2* own, int groups, const GclGeom& g, float eps) {
     __syncwarp();
     if (g.cluster > 1) { cluster_arrive(); cluster_wait(); } else __syncthreads();
-    for (int at = threadIdx.x; at < (groups * 8 + 31) / 32 * 32; at += kClusterThreads) {
+    for (int at = threadIdx.x; at < (groups * 8 + 31) / 32 * 32; at += THREADS) {
         const int group = at >> 3, r = at & 7;
         double s = 0.0, q = 0.0;
         if (group < groups && r < g.cluster) {
@@ -487,7 +490,7 @@ __global__ void __launch_bounds__(kClusterThreads) gcl_cluster_kernel(const T* x
     }
     __syncthreads();
     add_groups<kClusterThreads, Acc::D, V>(sums, g, slab0, slab, [&](int group, double s, double q) { mine[group][0] = s; mine[group][1] = q; });
-    join_cluster(mine, own, slab * V / g.per, g, eps);
+    join_cluster<kClusterThreads>(mine, own, slab * V / g.per, g, eps);
     if (live) {
         const int first = slab0 * V / g.per;
         float mean[V];
@@ -502,6 +505,84 @@ __global__ void __launch_bounds__(kClusterThreads) gcl_cluster_kernel(const T* x
     }
     __syncwarp();
     if (g.cluster > 1) cluster_wait();   // no CTA's memory goes while another reads it
+}
+
+// The same with the rows in shared memory: up to kResidentRows 16-byte vectors a thread (which alone reads what it copied, so
+// no barrier stands between), kResidentAhead batches of kResidentBatch on their way at a time.  A batch's rows are added while
+// later ones arrive.
+constexpr int kResidentRows = 26, kResidentBatch = 4, kResidentAhead = 4;
+static_assert(kResidentRows <= kRun, "one run of F32 sums");
+template <typename T, int ACT>
+__global__ void __launch_bounds__(kResidentThreads) gcl_resident_kernel(const T* x, const void* weight, int w_dt, const void* bias, int b_dt, T* out, GclGeom g,
+                                                                float eps, int kind) {
+    constexpr int V = 16 / sizeof(T), B = kResidentBatch;
+    using Acc = Sums<T, V, true>;
+    extern __shared__ __align__(16) uint4 resident_rows[];   // [row of the thread][thread]
+    __shared__ double sums[2][kResidentThreads];
+    __shared__ double mine[kClusterGroups][2];
+    __shared__ float2 own[kClusterGroups];
+    const int unit = blockIdx.x / g.cluster, rank = blockIdx.x - unit * g.cluster;
+    const int slabs = g.vectors / g.slab, b = unit / slabs, slab0 = (unit - b * slabs) * g.slab;
+    const int lane_vector = threadIdx.x % g.slab, lane_row = threadIdx.x / g.slab;
+    const int row0 = rank * g.rpp + lane_row, step = g.cluster * g.rpp, spatial = static_cast<int>(g.spatial);
+    const int rows = lane_row < g.rpp && row0 < spatial ? (spatial - 1 - row0) / step + 1 : 0;
+    const int64_t at0 = (static_cast<int64_t>(b) * g.spatial + row0) * g.channels + (slab0 + lane_vector) * V;
+    const int64_t p_step = static_cast<int64_t>(step) * g.channels;
+    const int c0 = (slab0 + lane_vector) * V;
+    const unsigned place = static_cast<unsigned>(__cvta_generic_to_shared(resident_rows + threadIdx.x));
+    pdl_wait();
+    auto copy = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < B; ++u)
+            if (i0 + u < rows)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(place + (i0 + u) * kResidentThreads * 16), "l"(x + at0 + (i0 + u) * p_step) : "memory");
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto row = [&](int i) {
+        const uint4 w = resident_rows[i * kResidentThreads + threadIdx.x];
+        Vec<T, V> v;
+        v.word[0] = w.x; v.word[1] = w.y; v.word[2] = w.z; v.word[3] = w.w;
+        return v;
+    };
+#pragma unroll
+    for (int i = 0; i < kResidentAhead; ++i) copy(i * B);
+    float scale[V], shift[V];
+    load_channels<V>(weight, w_dt, c0, g.row, 1.0f, scale);
+    load_channels<V>(bias, b_dt, c0, g.row, 0.0f, shift);
+    Acc acc;
+    acc.clear();
+#pragma unroll 1
+    for (int i = 0; i < rows; i += B) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kResidentAhead - 1) : "memory");
+        if (i == 0) acc.begin(row(0));
+#pragma unroll
+        for (int u = 0; u < B; ++u)
+            if (i + u < rows) acc.add(row(i + u));
+        copy(i + kResidentAhead * B);
+    }
+    if (rows > 0) acc.rebuild(rows);
+    sums[0][threadIdx.x] = acc.S[0];
+    sums[1][threadIdx.x] = acc.Q[0];
+    __syncthreads();
+    add_groups<kResidentThreads, 1, V>(sums, g, slab0, g.slab, [&](int group, double s, double q) { mine[group][0] = s; mine[group][1] = q; });
+    join_cluster<kResidentThreads>(mine, own, g.slab * V / g.per, g, eps);
+    if (rows > 0) {
+        const int first = slab0 * V / g.per;
+        float mean[V];
+        apply_stats<V>(g, c0, [&](int group) { return own[group - first]; }, mean, scale);
+#pragma unroll 1
+        for (int i = 0; i < rows; i += B) {
+#pragma unroll
+            for (int u = 0; u < B; ++u)
+                if (i + u < rows) {
+                    float y[V];
+                    normalise<ACT>(row(i + u), mean, scale, shift, kind, y);
+                    store_vec<V>(out + at0 + (i + u) * p_step, y);
+                }
+        }
+    }
+    __syncwarp();
+    if (g.cluster > 1) cluster_wait();
 }
 
 int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
@@ -553,9 +634,7 @@ void set_splits(GclGeom& g) {
 // more (a row's piece of a slab should fill memory sectors), its rows have to fit kMostRows rows of a thread in up to eight
 // CTAs, and all clusters should be at work at once.  Measured against the passes (bf16 with SiLU, back to back): 64 rows of 512
 // channels 4.9 us against 8.8, 256 rows 5.7 against 9.2, 2048 rows 8.0 against 11.8; with 16 rows a thread the code of a
-// once-run kernel costs more than a second read of x (4096 rows 15.9 against 12.6).  Keeping a slab's rows in the shared memory of
-// its cluster instead costs more too: pieces of 64 bytes of every row come at a quarter of the rate of whole rows (24960 rows
-// 32.2 against 20.2).
+// once-run kernel costs more than a second read of x (4096 rows 15.9 against 12.6).
 bool set_cluster(GclGeom& g, int v, int element) {
     int groups = 1;
     while (groups < g.groups && (groups * g.per % v != 0 || groups * g.per * element < 64 || g.groups % groups != 0)) ++groups;
@@ -570,6 +649,39 @@ bool set_cluster(GclGeom& g, int v, int element) {
     return passes <= static_cast<int64_t>(g.cluster) * kMostRows && g.batch * (g.vectors / g.slab) * g.cluster <= 4 * static_cast<int64_t>(sm_count());
 }
 
+// The slab and cluster of gcl_resident, or false: slabs of whole groups and of 16-byte vectors that lie in one group each, at
+// least 64 bytes or else 32 of every row, whose rows fit the shared memory of up to eight CTAs; all clusters at work at once, a CTA
+// to an SM, on half of the SMs or else a quarter (`room`: CTAs that fit for clusters of 1 to 8; a second wave costs as much as the
+// first).
+// Measured against the passes (bf16 with SiLU, back to back): 2400 rows of 512 channels 6.8 us against 11.6, 8000 rows 10.3 against
+// 13.1, 16000 rows 15.1 against 16.4; 4 x 4096 rows 12.7 against 16.1; 8 x 1035 rows of 320 channels in F32 7.8 against 18.4.
+// Pieces of 32 bytes come at half the rate: 20000 rows of 512 channels, 20 of a thread, 17.9 against 18.8, 24960 rows 20.4 against
+// 20.1, so those end at 20 rows.  On a quarter of the SMs: 3000 rows of 192 channels 7.1 against 9.6, 16384 of 128 10.1 against 10.9.
+bool set_resident(GclGeom& g, int v, int element, const int* room) {
+    if (v * element != 16 || !one_group(g, v) || g.spatial > INT32_MAX) return false;
+    for (int choice = 0; choice < 4; ++choice) {   // half of the SMs before a quarter, wide pieces before narrow ones
+        const int least = choice % 2 ? 32 : 64, share = choice < 2 ? 2 : 4;
+        int groups = 1;
+        while (groups < g.groups && (groups * g.per % v != 0 || groups * g.per * element < least || g.groups % groups != 0)) ++groups;
+        const int64_t slab = static_cast<int64_t>(groups) * g.per;
+        if (slab % v != 0 || slab / v > kResidentThreads || groups > kClusterGroups) continue;
+        g.vectors = g.channels / v;
+        g.slab = static_cast<int>(slab / v);
+        g.rpp = kResidentThreads / g.slab;
+        const int64_t passes = (g.spatial + g.rpp - 1) / g.rpp, most = least < 64 ? 20 : kResidentRows;
+        for (g.cluster = 8; g.cluster > 0; --g.cluster) {
+            const int64_t ctas = g.batch * (g.vectors / g.slab) * g.cluster;
+            if (g.cluster <= passes && passes <= most * g.cluster && ctas <= room[g.cluster] && ctas * share >= sm_count()) return true;
+        }
+    }
+    return false;
+}
+size_t resident_bytes(const GclGeom& g) {
+    const int64_t step = static_cast<int64_t>(g.cluster) * g.rpp;
+    return static_cast<size_t>((g.spatial + step - 1) / step) * kResidentThreads * 16;
+}
+constexpr size_t kResidentMost = static_cast<size_t>(kResidentRows) * kResidentThreads * 16;
+
 size_t up256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
 // the most any vector width asks for
 size_t partial_bytes(const GclGeom& g) {
@@ -581,10 +693,11 @@ size_t workspace_size(const GclGeom& g) {
 }
 
 template <typename... KArgs, typename... Args>
-void launch_clusters(void (*kernel)(KArgs...), unsigned ctas, int cluster, cudaStream_t stream, Args&&... args) {
+void launch_clusters(void (*kernel)(KArgs...), unsigned ctas, int threads, size_t shared, int cluster, cudaStream_t stream, Args&&... args) {
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(ctas);
-    config.blockDim = dim3(kClusterThreads);
+    config.blockDim = dim3(static_cast<unsigned>(threads));
+    config.dynamicSmemBytes = shared;
     config.stream = stream;
     cudaLaunchAttribute attributes[2];
     attributes[0].id = cudaLaunchAttributeClusterDimension;
@@ -607,7 +720,7 @@ struct GclCall {
 template <typename T, int V, bool WHOLE, int ACT>
 int run_cluster(const GclCall& c, const GclGeom& g, cudaStream_t s) {
     const int64_t units = g.batch * ((g.vectors + g.slab - 1) / g.slab);
-    launch_clusters(gcl_cluster_kernel<T, V, WHOLE, ACT>, static_cast<unsigned>(units * g.cluster), g.cluster, s, static_cast<const T*>(c.x), c.weight, c.w_dt, c.bias,
+    launch_clusters(gcl_cluster_kernel<T, V, WHOLE, ACT>, static_cast<unsigned>(units * g.cluster), kClusterThreads, 0, g.cluster, s, static_cast<const T*>(c.x), c.weight, c.w_dt, c.bias,
                     c.b_dt, static_cast<T*>(c.out), g, c.eps, c.activation);
     return after_launch("group_norm_channels_last");
 }
@@ -617,6 +730,22 @@ int run_cluster(const GclCall& c, const GclGeom& g, cudaStream_t s) {
     if (c.activation == VRB_SILU) return run_cluster<T, V, WHOLE, 1>(c, g, s);
     if (c.activation == VRB_GELU_TANH) return run_cluster<T, V, WHOLE, 2>(c, g, s);
     return run_cluster<T, V, WHOLE, 3>(c, g, s);
+}
+
+template <typename T, int ACT>
+int run_resident(const GclCall& c, const GclGeom& g, cudaStream_t s) {
+    static std::atomic<uint64_t> allowed{0};
+    if (int rc = allow_shared(gcl_resident_kernel<T, ACT>, kResidentMost, allowed, "group_norm_channels_last")) return rc;
+    launch_clusters(gcl_resident_kernel<T, ACT>, static_cast<unsigned>(g.batch * (g.vectors / g.slab) * g.cluster), kResidentThreads, resident_bytes(g), g.cluster, s,
+                    static_cast<const T*>(c.x), c.weight, c.w_dt, c.bias, c.b_dt, static_cast<T*>(c.out), g, c.eps, c.activation);
+    return after_launch("group_norm_channels_last");
+}
+template <typename T>
+int run_resident(const GclCall& c, const GclGeom& g, cudaStream_t s) {
+    if (c.activation == VRB_NO_ACTIVATION) return run_resident<T, 0>(c, g, s);
+    if (c.activation == VRB_SILU) return run_resident<T, 1>(c, g, s);
+    if (c.activation == VRB_GELU_TANH) return run_resident<T, 2>(c, g, s);
+    return run_resident<T, 3>(c, g, s);
 }
 
 template <typename T, int V>
@@ -697,13 +826,17 @@ extern "C" int vrb_group_norm_channels_last(const void* x, int dtype, const void
     int v = vector_width(dtype, batch, spatial, channels, groups, false, x, out);
     GclGeom h = g;
     const bool cluster = set_cluster(h, v, static_cast<int>(dtype_bytes(dtype)));
-    if (!cluster) v = vector_width(dtype, batch, spatial, channels, groups, true, x, out);
-    const size_t need = cluster ? 0 : workspace_size(g);
+    GclGeom r = g;
+    const bool resident = !cluster && set_resident(r, v, static_cast<int>(dtype_bytes(dtype)),
+                                                   cluster_room(reinterpret_cast<const void*>(gcl_resident_kernel<uint16_t, 0>), kResidentThreads, kResidentMost));
+    if (!cluster && !resident) v = vector_width(dtype, batch, spatial, channels, groups, true, x, out);
+    const size_t need = cluster || resident ? 0 : workspace_size(g);
     VRB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0), VRB_ERR_WORKSPACE,
                 "group_norm_channels_last: workspace needs %zu bytes, 256-byte aligned", need);
     char* ws = static_cast<char*>(workspace);
     cudaStream_t s = as_stream(stream);
     const GclCall c{x, weight, bias, out, weight_dtype, bias_dtype, activation, eps};
+    if (resident) return dtype == VRB_BF16 ? run_resident<uint16_t>(c, r, s) : run_resident<float>(c, r, s);
     if (dtype == VRB_BF16) {
         if (v == 8) return run_width<uint16_t, 8>(c, g, cluster, ws, s);
         if (v == 4) return run_width<uint16_t, 4>(c, g, cluster, ws, s);

@@ -21,6 +21,39 @@ void* tensor_map_encoder() {
     return encoder;
 }
 
+const int* cluster_room(const void* kernel, int threads, size_t most_shared) {
+    static std::atomic<int> known[64][kMostCluster + 1];
+    static thread_local int room[kMostCluster + 1];
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) device = 0;
+    for (int cluster = 1; cluster <= kMostCluster; ++cluster) {
+        int n = known[device][cluster].load(std::memory_order_relaxed);
+        if (n == 0) {
+            n = sm_count();
+            if (cluster > 1) {
+                cudaLaunchConfig_t config = {};
+                config.gridDim = dim3(static_cast<unsigned>(n / cluster * cluster));
+                config.blockDim = dim3(static_cast<unsigned>(threads));
+                config.dynamicSmemBytes = 120 * 1024;   // one CTA to an SM
+                cudaLaunchAttribute attribute;
+                attribute.id = cudaLaunchAttributeClusterDimension;
+                attribute.val.clusterDim.x = static_cast<unsigned>(cluster);
+                attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+                config.attrs = &attribute;
+                config.numAttrs = 1;
+                int clusters = 0;
+                const bool asked = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most_shared)) == cudaSuccess &&
+                                   cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) == cudaSuccess && clusters > 0;
+                if (!asked) cudaGetLastError();
+                n = asked ? clusters * cluster : n * 3 / 4;
+            }
+            known[device][cluster].store(n, std::memory_order_relaxed);
+        }
+        room[cluster] = n;
+    }
+    return room;
+}
+
 bool encode_tile_map(CUtensorMap* map, const void* base, int dtype, int64_t outer, int64_t channels, int64_t inner,
                      int box_inner, int box_channels) {
     using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
