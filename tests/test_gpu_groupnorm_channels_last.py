@@ -208,6 +208,74 @@ def test_repeats_captures_and_streams(gpu):
     assert all(torch.equal(outs[i], want[i]) for i in range(3))
 
 
+def test_middle_maps_bad_values_and_alignment(gpu):
+    """An infinity or a NaN spoils its own group only; a map off the 16-byte boundaries takes another way to the same bound."""
+    import torch
+    be, ops = gpu
+    for dtype in (torch.bfloat16, torch.float32):
+        x, w, b = _make((1, 4100, 512), dtype, 8)
+        clean = be.group_norm_channels_last(x, 32, w, b, 1e-6, activation=ops.SILU)
+        shifted = torch.empty(x.numel() + 1, device="cuda", dtype=dtype)[1:].view(x.shape)
+        shifted.copy_(x)
+        _check(be.group_norm_channels_last(shifted, 32, w, b, 1e-6, activation=ops.SILU), x, 32, w, b, 1e-6, ops.SILU)
+        x[0, 4099, 33] = float("nan")
+        x[0, 5, 500] = float("inf")
+        y = be.group_norm_channels_last(x, 32, w, b, 1e-6, activation=ops.SILU)
+        bad = torch.zeros_like(y, dtype=torch.bool)
+        bad[0, :, 32:48] = True
+        bad[0, :, 496:512] = True
+        assert torch.equal(y[~bad], clean[~bad]) and torch.isnan(y[bad]).all()
+
+
+def test_middle_maps_together(gpu):
+    """Clusters that each want a whole SM, from four streams at once, eager and replayed."""
+    import torch
+    be, ops = gpu
+    shapes = [((1, 4096, 512), 32), ((4, 4096, 128), 8), ((1, 16000, 512), 32), ((8, 1035, 320), 8)]
+    data = [_make(s, torch.bfloat16, 20 + i) for i, (s, _) in enumerate(shapes)]
+    want = [be.group_norm_channels_last(x, g, w, b, 1e-6) for (x, w, b), (_, g) in zip(data, shapes)]
+    graphs, outs = [], []
+    for (x, w, b), (_, g) in zip(data, shapes):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(be.group_norm_channels_last(x, g, w, b, 1e-6))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in shapes]
+    torch.cuda.synchronize()
+    eager = []
+    for _ in range(10):
+        for i, ((x, w, b), (_, g)) in enumerate(zip(data, shapes)):
+            with torch.cuda.stream(streams[i]):
+                eager.append((i, be.group_norm_channels_last(x, g, w, b, 1e-6)))
+                graphs[i].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i, y in eager) and all(torch.equal(y, z) for y, z in zip(outs, want))
+
+
+def test_first_call_of_a_process_is_captured(gpu):
+    """No call of the library before the capture: room for clusters and shared memory are asked for while capturing."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from vrhino_b200 import ops
+be = ops.B200Backend()
+x = torch.randn((1, 5000, 512), device="cuda").bfloat16()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = be.group_norm_channels_last(x, 32, None, None, 1e-6, activation=0)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(y, be.group_norm_channels_last(x, 32, None, None, 1e-6, activation=0))
+print("captured")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=root, timeout=120)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
+
+
 def test_past_32_bit_offsets(gpu):
     import torch
     be, ops = gpu
