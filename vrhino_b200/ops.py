@@ -655,7 +655,7 @@ class B200Backend:
         spatial = count // (batch * channels)
         need = _channels_last_workspace(device.index, code, batch, spatial, channels, groups)
         # scratch of this call alone: torch's allocator keeps it from other streams and other captured graphs
-        scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        scratch = x.new_empty(need, dtype=torch.uint8) if need else None
         _launch("vrb_group_norm_channels_last", device, x.data_ptr(), code, _address(weight, device), 0 if weight is None else _code(weight),
                 _address(bias, device), 0 if bias is None else _code(bias), out.data_ptr(), batch, spatial, channels, groups, eps,
                 _lib.NO_ACTIVATION if activation is None else int(activation), scratch.data_ptr() if need else None, need)
@@ -685,8 +685,8 @@ class B200Backend:
         k = shape[-1]
         rows = count // k
         if out is None:
-            codes = torch.empty((rows, (k + 31) // 32 * 16), dtype=torch.uint8, device=device)
-            scales = torch.empty((rows + 127) // 128 * ((k + span - 1) // span) * 512, dtype=torch.uint8, device=device)
+            codes = x.new_empty((rows, (k + 31) // 32 * 16), dtype=torch.uint8)
+            scales = codes.new_empty((rows + 127) // 128 * ((k + span - 1) // span) * 512)
             out = Fp4Tensor(codes, scales, tensor_scale, format, shape)
             codes, scales, scale = codes.data_ptr(), scales.data_ptr(), _fp4_scale_address(tensor_scale, device)
         elif out.format != format or out.tensor_scale is not tensor_scale or tuple(out.shape) != shape or out.codes.device != device:
@@ -717,7 +717,7 @@ class B200Backend:
         if bias is not None and bias.numel() != n:
             raise VrbError("linear bias mismatch")
         shape = tuple(x.shape[:-1]) + (n,)
-        out = torch.empty(shape, dtype=dtype, device=device) if out is None else _result(out, shape, dtype, device)
+        out = x.codes.new_empty(shape, dtype=dtype) if out is None else _result(out, shape, dtype, device)
         _launch("vrb_fp4_linear", device, x.format, a_codes, a_scales, a_scale, m, b_codes, b_scales, b_scale, n, k, _address(bias, device),
                 0 if bias is None else _code(bias), _lib.NO_ACTIVATION if activation is None else int(activation), out.data_ptr(), _code(dtype))
         return out
