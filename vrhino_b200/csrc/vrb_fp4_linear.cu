@@ -658,8 +658,8 @@ int launch_pair(const LinearMaps& maps, const LinearArgs& p, cudaStream_t s) {
     return after_launch("fp4_linear");
 }
 // Which kernel, and the split kernel's tile and cluster: the least of the times that a model gives, in nanoseconds, fitted to
-// both kernels on B200 (back to back in a graph; the choice is within 3 % of the best on 24 shapes between 1 x 512 x 512
-// and 4000 x 6000 x 30720).  Pair kernel: 4300 + 500 a tile + 290 a stage.  Split kernel: 2300 + 19 a column
+// both kernels on B200 (back to back in a graph; the choice is within 3 % of the best on 24 shapes from 1 x 512 x 512
+// to 4000 x 6000 and to k past 30000).  Pair kernel: 4300 + 500 a tile + 290 a stage.  Split kernel: 2300 + 19 a column
 // of the tile + 265 a stage, and 800 + 130 a CTA to meet in a cluster; one CTA to an SM, what does not fit at once takes turns.
 struct LinearPlan {
     int columns;   // 0: pair kernel
