@@ -66,6 +66,8 @@ SHAPES = [
 MIDDLE = [
     ((1, 4097, 512), 32), ((1, 24960, 512), 32), ((1, 26624, 256), 16), ((1, 26625, 256), 16), ((2, 1100, 320), 32), ((1, 9216, 320), 32),
     ((1, 1500, 2048), 16), ((1, 12000, 32), 1), ((3, 6000, 128), 8), ((1, 5001, 96), 2), ((1, 9999, 192), 6), ((2, 5300, 64), 1),
+    # groups of an even number of channels that is no multiple of a vector's, small to large
+    ((3, 1035, 320), 32), ((8, 1035, 320), 32), ((2, 4099, 320), 32), ((2, 1030, 640), 32), ((1, 30001, 96), 16), ((1, 50001, 30), 15), ((1, 40001, 24), 4),
 ]
 
 

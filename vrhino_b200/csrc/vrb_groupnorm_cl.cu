@@ -114,11 +114,11 @@ __device__ __forceinline__ void normalise(const Vec<T, V>& v, const float (&mean
     }
 }
 
-// Sums of a thread's V channels over a run, and what has been rebuilt from earlier runs.  WHOLE: the V channels lie in one group
+// Sums of a thread's V channels over a run, and what has been rebuilt from earlier runs.  E consecutive channels lie in one group
 // and share the double sums.
-template <typename T, int V, bool WHOLE>
+template <typename T, int V, int E>
 struct Sums {
-    static constexpr int D = WHOLE ? 1 : V;
+    static constexpr int D = V / E;
     double S[D], Q[D];
     float K[V], s1[V], s2[V];
     __device__ __forceinline__ void clear() {
@@ -145,15 +145,15 @@ struct Sums {
     }
     __device__ __forceinline__ void single(int e, float v) {
         const double d = v;
-        S[WHOLE ? 0 : e] += d;
-        Q[WHOLE ? 0 : e] += d * d;
+        S[e / E] += d;
+        Q[e / E] += d * d;
     }
     __device__ __forceinline__ void rebuild(int n) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             const double k = K[e], nk = n * k;
-            S[WHOLE ? 0 : e] += s1[e] + nk;
-            Q[WHOLE ? 0 : e] += s2[e] + k * (2.0 * s1[e] + nk);
+            S[e / E] += s1[e] + nk;
+            Q[e / E] += s2[e] + k * (2.0 * s1[e] + nk);
         }
     }
 };
@@ -194,9 +194,9 @@ __device__ __forceinline__ float2 moments_to_stats(double s, double q, double sh
 }
 
 // partial[((b * splits + split) * groups + g) * 2 + {0, 1}] = {sum x, sum x^2} over the CTA's rows.  One CTA to an SM.
-template <typename T, int V, bool WHOLE>
+template <typename T, int V, int E>
 __global__ void __launch_bounds__(kThreads, 1) gcl_partial_kernel(const T* x, double* __restrict__ partial, GclGeom g) {
-    using Acc = Sums<T, V, WHOLE>;
+    using Acc = Sums<T, V, E>;
     __shared__ double sums[2][kThreads * Acc::D];
     pdl_wait();
     const int b = blockIdx.x / g.splits, split = blockIdx.x - b * g.splits;
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, 1) gcl_partial_kernel(const T* x, do
         Acc acc;
         acc.clear();
         if (lane_row < g.rpp && lane_vector < slab) {
-            constexpr int U = WHOLE && sizeof(T) * V == 16 ? 8 : 4;
+            constexpr int U = E == V && sizeof(T) * V == 16 ? 8 : 4;
             const int64_t step = static_cast<int64_t>(g.splits) * g.rpp, p_step = step * g.channels;
             const int64_t row = static_cast<int64_t>(split) * g.rpp + lane_row;
             const T* p = x + b * g.entry + row * g.channels + (slab0 + lane_vector) * V;
@@ -446,10 +446,10 @@ __device__ __forceinline__ void join_cluster(const double (*mine)[2], float2* ow
 // One cluster per (batch entry, slab of whole groups): up to kMostRows rows of a thread stay in registers between the statistics
 // and the result.  Row i of a thread is (i * cluster + rank) * rpp + lane_row.
 constexpr int kMostRows = 4;
-template <typename T, int V, bool WHOLE, int ACT>
+template <typename T, int V, int E, int ACT>
 __global__ void __launch_bounds__(kClusterThreads) gcl_cluster_kernel(const T* x, const void* weight, int w_dt, const void* bias, int b_dt, T* out, GclGeom g,
                                                               float eps, int kind) {
-    using Acc = Sums<T, V, WHOLE>;
+    using Acc = Sums<T, V, E>;
     __shared__ double sums[2][kClusterThreads * Acc::D];
     __shared__ double mine[kClusterGroups][2];
     __shared__ float2 own[kClusterGroups];
@@ -507,18 +507,19 @@ __global__ void __launch_bounds__(kClusterThreads) gcl_cluster_kernel(const T* x
     if (g.cluster > 1) cluster_wait();   // no CTA's memory goes while another reads it
 }
 
-// The same with the rows in shared memory: up to kResidentRows 16-byte vectors a thread (which alone reads what it copied, so
+// The same with the rows in shared memory: up to most_resident_rows() 16-byte vectors a thread (which alone reads what it copied, so
 // no barrier stands between), kResidentAhead batches of kResidentBatch on their way at a time.  A batch's rows are added while
 // later ones arrive.
-constexpr int kResidentRows = 26, kResidentBatch = 4, kResidentAhead = 4;
-static_assert(kResidentRows <= kRun, "one run of F32 sums");
-template <typename T, int ACT>
+constexpr int kResidentBatch = 4, kResidentAhead = 4;
+constexpr int most_resident_rows(int entries) { return 27 - entries; }   // with the double sums of `entries` (1, 2 or 4) a thread: 219 KB
+static_assert(most_resident_rows(1) <= kRun, "one run of F32 sums");
+template <typename T, int E, int ACT>
 __global__ void __launch_bounds__(kResidentThreads) gcl_resident_kernel(const T* x, const void* weight, int w_dt, const void* bias, int b_dt, T* out, GclGeom g,
                                                                 float eps, int kind) {
     constexpr int V = 16 / sizeof(T), B = kResidentBatch;
-    using Acc = Sums<T, V, true>;
+    using Acc = Sums<T, V, E>;
     extern __shared__ __align__(16) uint4 resident_rows[];   // [row of the thread][thread]
-    __shared__ double sums[2][kResidentThreads];
+    __shared__ double sums[2][kResidentThreads * Acc::D];
     __shared__ double mine[kClusterGroups][2];
     __shared__ float2 own[kClusterGroups];
     const int unit = blockIdx.x / g.cluster, rank = blockIdx.x - unit * g.cluster;
@@ -561,10 +562,13 @@ __global__ void __launch_bounds__(kResidentThreads) gcl_resident_kernel(const T*
         copy(i + kResidentAhead * B);
     }
     if (rows > 0) acc.rebuild(rows);
-    sums[0][threadIdx.x] = acc.S[0];
-    sums[1][threadIdx.x] = acc.Q[0];
+#pragma unroll
+    for (int e = 0; e < Acc::D; ++e) {
+        sums[0][threadIdx.x * Acc::D + e] = acc.S[e];
+        sums[1][threadIdx.x * Acc::D + e] = acc.Q[e];
+    }
     __syncthreads();
-    add_groups<kResidentThreads, 1, V>(sums, g, slab0, g.slab, [&](int group, double s, double q) { mine[group][0] = s; mine[group][1] = q; });
+    add_groups<kResidentThreads, Acc::D, V>(sums, g, slab0, g.slab, [&](int group, double s, double q) { mine[group][0] = s; mine[group][1] = q; });
     join_cluster<kResidentThreads>(mine, own, g.slab * V / g.per, g, eps);
     if (rows > 0) {
         const int first = slab0 * V / g.per;
@@ -588,19 +592,23 @@ __global__ void __launch_bounds__(kResidentThreads) gcl_resident_kernel(const T*
 int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
 // Elements of a vector: the most, up to 16 bytes, for which every batch entry begins on a vector's boundary; rows that are no
 // multiple of it are folded where the folded row is not too long for a CTA.  Eight bf16 channels only where they lie in one
-// group: eight pairs of double sums a thread are more than the registers take.
+// group or two by two: eight pairs of double sums a thread are more than the registers take.
 int vector_width(int dtype, int64_t batch, int64_t spatial, int64_t channels, int groups, bool fold, const void* x, const void* out) {
     const int element = static_cast<int>(dtype_bytes(dtype));
     for (int v = 16 / element; v > 1; v /= 2) {
         const int64_t folded = channels / gcd(static_cast<int>(channels), v);
         if (channels % v != 0 && (!fold || folded > kThreads || spatial < v || (batch > 1 && spatial * channels % v != 0))) continue;
-        if (v == 8 && groups > 1 && channels / groups % 8 != 0) continue;
+        if (v == 8 && groups > 1 && (channels % 2 != 0 || channels / groups % 2 != 0)) continue;
         if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) % (v * element) == 0) return v;
     }
     return 1;
 }
-// Whether the V channels of a vector always lie in one group
-bool one_group(const GclGeom& g, int v) { return g.groups == 1 || (g.row % v == 0 && g.per % v == 0); }
+// Consecutive channels of a vector that always lie in one group and share their double sums: all, two or one.  (Two rather than
+// one: 300000 rows of 160 channels in groups of 10, bf16 with SiLU, 58.7 us against 69.6, 3 x 1035 of 320 5.9 against 17.3.)
+int entry_channels(const GclGeom& g, int v) {
+    if (g.groups == 1 || (g.row % v == 0 && g.per % v == 0)) return v;
+    return v > 2 && g.row % 2 == 0 && g.per % 2 == 0 ? 2 : 1;
+}
 
 int make_geom(GclGeom& g, int64_t batch, int64_t spatial, int64_t channels, int groups) {
     VRB_REQUIRE(batch > 0 && spatial > 0 && channels > 0 && groups > 0 && channels % groups == 0, VRB_ERR_INVALID,
@@ -649,16 +657,17 @@ bool set_cluster(GclGeom& g, int v, int element) {
     return passes <= static_cast<int64_t>(g.cluster) * kMostRows && g.batch * (g.vectors / g.slab) * g.cluster <= 4 * static_cast<int64_t>(sm_count());
 }
 
-// The slab and cluster of gcl_resident, or false: slabs of whole groups and of 16-byte vectors that lie in one group each, at
-// least 64 bytes or else 32 of every row, whose rows fit the shared memory of up to eight CTAs; all clusters at work at once, a CTA
-// to an SM, on half of the SMs or else a quarter (`room`: CTAs that fit for clusters of 1 to 8; a second wave costs as much as the
-// first).
-// Measured against the passes (bf16 with SiLU, back to back): 2400 rows of 512 channels 6.8 us against 11.6, 8000 rows 10.3 against
-// 13.1, 16000 rows 15.1 against 16.4; 4 x 4096 rows 12.7 against 16.1; 8 x 1035 rows of 320 channels in F32 7.8 against 18.4.
-// Pieces of 32 bytes come at half the rate: 20000 rows of 512 channels, 20 of a thread, 17.9 against 18.8, 24960 rows 20.4 against
-// 20.1, so those end at 20 rows.  On a quarter of the SMs: 3000 rows of 192 channels 7.1 against 9.6, 16384 of 128 10.1 against 10.9.
+// The slab and cluster of gcl_resident, or false: slabs of whole groups and of 16-byte vectors (whose channels lie in one group or
+// two by two), at least 64 bytes or else 32 of every row, whose rows fit the shared memory of up to eight CTAs; all clusters at work
+// at once, a CTA to an SM, on half of the SMs or else a quarter (`room`: CTAs that fit for clusters of 1 to 8; a second wave costs
+// as much as the first).  Measured against the passes (bf16 with SiLU, back to back): 2400 rows of 512 channels 6.8 us against 11.6,
+// 8000 rows 10.3 against 13.1, 16000 rows 15.1 against 16.4; 4 x 4096 rows 12.7 against 16.1; 8 x 4096 rows of 320 channels 17.3
+// against 34.1.  Pieces of 32 bytes come at half the rate: 20000 rows of 512 channels, 20 of a thread, 17.9 against 18.8, 24960 rows
+// 20.4 against 20.1, so those end at 20 rows.  On a quarter of the SMs: 3000 rows of 192 channels, 3 of a thread, 7.1 against 9.6,
+// 16384 of 128, 8 of a thread, 10.1 against 10.9, 9216 of 320, 12 of a thread, 12.7 against 12.3.
 bool set_resident(GclGeom& g, int v, int element, const int* room) {
-    if (v * element != 16 || !one_group(g, v) || g.spatial > INT32_MAX) return false;
+    const int entries = v / entry_channels(g, v);
+    if (v * element != 16 || entries > 4 || (entries > 2 && element == 4) || g.spatial > INT32_MAX) return false;
     for (int choice = 0; choice < 4; ++choice) {   // half of the SMs before a quarter, wide pieces before narrow ones
         const int least = choice % 2 ? 32 : 64, share = choice < 2 ? 2 : 4;
         int groups = 1;
@@ -668,7 +677,7 @@ bool set_resident(GclGeom& g, int v, int element, const int* room) {
         g.vectors = g.channels / v;
         g.slab = static_cast<int>(slab / v);
         g.rpp = kResidentThreads / g.slab;
-        const int64_t passes = (g.spatial + g.rpp - 1) / g.rpp, most = least < 64 ? 20 : kResidentRows;
+        const int64_t passes = (g.spatial + g.rpp - 1) / g.rpp, most = share > 2 ? 8 : least < 64 ? 20 : most_resident_rows(entries);
         for (g.cluster = 8; g.cluster > 0; --g.cluster) {
             const int64_t ctas = g.batch * (g.vectors / g.slab) * g.cluster;
             if (g.cluster <= passes && passes <= most * g.cluster && ctas <= room[g.cluster] && ctas * share >= sm_count()) return true;
@@ -680,7 +689,7 @@ size_t resident_bytes(const GclGeom& g) {
     const int64_t step = static_cast<int64_t>(g.cluster) * g.rpp;
     return static_cast<size_t>((g.spatial + step - 1) / step) * kResidentThreads * 16;
 }
-constexpr size_t kResidentMost = static_cast<size_t>(kResidentRows) * kResidentThreads * 16;
+constexpr size_t resident_most(int entries) { return static_cast<size_t>(most_resident_rows(entries)) * kResidentThreads * 16; }
 
 size_t up256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
 // the most any vector width asks for
@@ -717,35 +726,40 @@ struct GclCall {
     float eps;
 };
 
-template <typename T, int V, bool WHOLE, int ACT>
+template <typename T, int V, int E, int ACT>
 int run_cluster(const GclCall& c, const GclGeom& g, cudaStream_t s) {
     const int64_t units = g.batch * ((g.vectors + g.slab - 1) / g.slab);
-    launch_clusters(gcl_cluster_kernel<T, V, WHOLE, ACT>, static_cast<unsigned>(units * g.cluster), kClusterThreads, 0, g.cluster, s, static_cast<const T*>(c.x), c.weight, c.w_dt, c.bias,
+    launch_clusters(gcl_cluster_kernel<T, V, E, ACT>, static_cast<unsigned>(units * g.cluster), kClusterThreads, 0, g.cluster, s, static_cast<const T*>(c.x), c.weight, c.w_dt, c.bias,
                     c.b_dt, static_cast<T*>(c.out), g, c.eps, c.activation);
     return after_launch("group_norm_channels_last");
 }
-template <typename T, int V, bool WHOLE>
+template <typename T, int V, int E>
 int run_cluster(const GclCall& c, const GclGeom& g, cudaStream_t s) {
-    if (c.activation == VRB_NO_ACTIVATION) return run_cluster<T, V, WHOLE, 0>(c, g, s);
-    if (c.activation == VRB_SILU) return run_cluster<T, V, WHOLE, 1>(c, g, s);
-    if (c.activation == VRB_GELU_TANH) return run_cluster<T, V, WHOLE, 2>(c, g, s);
-    return run_cluster<T, V, WHOLE, 3>(c, g, s);
+    if (c.activation == VRB_NO_ACTIVATION) return run_cluster<T, V, E, 0>(c, g, s);
+    if (c.activation == VRB_SILU) return run_cluster<T, V, E, 1>(c, g, s);
+    if (c.activation == VRB_GELU_TANH) return run_cluster<T, V, E, 2>(c, g, s);
+    return run_cluster<T, V, E, 3>(c, g, s);
 }
 
-template <typename T, int ACT>
+template <typename T, int E, int ACT>
 int run_resident(const GclCall& c, const GclGeom& g, cudaStream_t s) {
     static std::atomic<uint64_t> allowed{0};
-    if (int rc = allow_shared(gcl_resident_kernel<T, ACT>, kResidentMost, allowed, "group_norm_channels_last")) return rc;
-    launch_clusters(gcl_resident_kernel<T, ACT>, static_cast<unsigned>(g.batch * (g.vectors / g.slab) * g.cluster), kResidentThreads, resident_bytes(g), g.cluster, s,
+    if (int rc = allow_shared(gcl_resident_kernel<T, E, ACT>, resident_most(static_cast<int>(16 / sizeof(T)) / E), allowed, "group_norm_channels_last")) return rc;
+    launch_clusters(gcl_resident_kernel<T, E, ACT>, static_cast<unsigned>(g.batch * (g.vectors / g.slab) * g.cluster), kResidentThreads, resident_bytes(g), g.cluster, s,
                     static_cast<const T*>(c.x), c.weight, c.w_dt, c.bias, c.b_dt, static_cast<T*>(c.out), g, c.eps, c.activation);
     return after_launch("group_norm_channels_last");
 }
+template <typename T, int E>
+int run_resident(const GclCall& c, const GclGeom& g, cudaStream_t s) {
+    if (c.activation == VRB_NO_ACTIVATION) return run_resident<T, E, 0>(c, g, s);
+    if (c.activation == VRB_SILU) return run_resident<T, E, 1>(c, g, s);
+    if (c.activation == VRB_GELU_TANH) return run_resident<T, E, 2>(c, g, s);
+    return run_resident<T, E, 3>(c, g, s);
+}
 template <typename T>
 int run_resident(const GclCall& c, const GclGeom& g, cudaStream_t s) {
-    if (c.activation == VRB_NO_ACTIVATION) return run_resident<T, 0>(c, g, s);
-    if (c.activation == VRB_SILU) return run_resident<T, 1>(c, g, s);
-    if (c.activation == VRB_GELU_TANH) return run_resident<T, 2>(c, g, s);
-    return run_resident<T, 3>(c, g, s);
+    constexpr int V = 16 / sizeof(T);
+    return entry_channels(g, V) == V ? run_resident<T, V>(c, g, s) : run_resident<T, 2>(c, g, s);
 }
 
 template <typename T, int V>
@@ -756,8 +770,12 @@ int run_passes(const GclCall& c, GclGeom g, char* workspace, cudaStream_t s) {
     float2* stats = g.groups > kInlineGroups ? reinterpret_cast<float2*>(workspace + partial_bytes(g)) : nullptr;
     const dim3 ctas_stats(static_cast<unsigned>(g.batch * g.splits));
     const T* x = static_cast<const T*>(c.x);
-    if (one_group(g, V)) launch_overlapped(gcl_partial_kernel<T, V, true>, ctas_stats, dim3(kThreads), 0, s, x, partial, g);
-    else if constexpr (V > 1 && V < 8) launch_overlapped(gcl_partial_kernel<T, V, false>, ctas_stats, dim3(kThreads), 0, s, x, partial, g);
+    const int entry = entry_channels(g, V);
+    if (entry == V) launch_overlapped(gcl_partial_kernel<T, V, V>, ctas_stats, dim3(kThreads), 0, s, x, partial, g);
+    if constexpr (V > 2)
+        if (entry == 2) launch_overlapped(gcl_partial_kernel<T, V, 2>, ctas_stats, dim3(kThreads), 0, s, x, partial, g);
+    if constexpr (V > 1 && V < 8)
+        if (entry == 1) launch_overlapped(gcl_partial_kernel<T, V, 1>, ctas_stats, dim3(kThreads), 0, s, x, partial, g);
     if (int rc = after_launch("group_norm_channels_last statistics")) return rc;
     if (stats) {
         launch_overlapped(gcl_finalize_kernel, dim3(static_cast<unsigned>(g.batch * ((g.groups + kFinalizeGroups - 1) / kFinalizeGroups))), dim3(kThreads), 0, s, partial,
@@ -785,9 +803,12 @@ template <typename T, int V>
 int run_width(const GclCall& c, GclGeom g, bool cluster, char* workspace, cudaStream_t s) {
     if (!cluster) return run_passes<T, V>(c, g, workspace, s);
     set_cluster(g, V, sizeof(T));
+    const int entry = entry_channels(g, V);
+    if constexpr (V > 2)
+        if (entry == 2) return run_cluster<T, V, 2>(c, g, s);
     if constexpr (V > 1 && V < 8)
-        if (!one_group(g, V)) return run_cluster<T, V, false>(c, g, s);
-    return run_cluster<T, V, true>(c, g, s);
+        if (entry == 1) return run_cluster<T, V, 1>(c, g, s);
+    return run_cluster<T, V, V>(c, g, s);
 }
 
 }  // namespace
@@ -803,7 +824,7 @@ extern "C" size_t vrb_group_norm_channels_last_workspace_bytes(int dtype, int64_
     bool cluster = true;
     for (int v = 16 / element; v >= 1 && cluster; v /= 2) {
         GclGeom h = g;
-        if (channels % v == 0 && (v < 8 || groups == 1 || h.per % 8 == 0)) cluster = set_cluster(h, v, element);
+        if (channels % v == 0 && (v < 8 || groups == 1 || h.per % 2 == 0)) cluster = set_cluster(h, v, element);
     }
     return cluster ? 0 : workspace_size(g);
 }
@@ -828,7 +849,7 @@ extern "C" int vrb_group_norm_channels_last(const void* x, int dtype, const void
     const bool cluster = set_cluster(h, v, static_cast<int>(dtype_bytes(dtype)));
     GclGeom r = g;
     const bool resident = !cluster && set_resident(r, v, static_cast<int>(dtype_bytes(dtype)),
-                                                   cluster_room(reinterpret_cast<const void*>(gcl_resident_kernel<uint16_t, 0>), kResidentThreads, kResidentMost));
+                                                   cluster_room(reinterpret_cast<const void*>(gcl_resident_kernel<uint16_t, 8, 0>), kResidentThreads, resident_most(1)));
     if (!cluster && !resident) v = vector_width(dtype, batch, spatial, channels, groups, true, x, out);
     const size_t need = cluster || resident ? 0 : workspace_size(g);
     VRB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0), VRB_ERR_WORKSPACE,
