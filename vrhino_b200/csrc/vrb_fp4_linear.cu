@@ -77,6 +77,12 @@ __device__ __forceinline__ bool wait_barrier(uint64_t* barrier, unsigned parity,
         }
     }
 }
+// The same for a whole warp, with one outcome for all lanes: lanes may meet the limit or another warp's abort apart from each
+// other, and what follows a wait (elect.sync, __syncwarp, aligned tensor-memory reads) needs all of them.  The vote costs the
+// pair kernel 1 to 2 % (32760 x 1536 x 8960 with GELU 301 -> 306 us among passes); a single thread for each loop cost 2 to 4.
+__device__ __forceinline__ bool wait_warp(uint64_t* barrier, unsigned parity, volatile int* abort) {
+    return __all_sync(0xffffffffu, wait_barrier(barrier, parity, abort));
+}
 __device__ __forceinline__ unsigned cluster_rank() {
     unsigned r;
     asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
@@ -297,7 +303,7 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
             unsigned row_tile, column_tile;
             tile_of(t, row_tiles, column_tiles, row_tile, column_tile);
             for (int stage = 0; stage < stages; ++stage) {
-                if (!wait_barrier(&control.empty[slot], phase, &control.abort)) { ok = false; break; }
+                if (!wait_warp(&control.empty[slot], phase, &control.abort)) { ok = false; break; }
                 if (elect_one()) {
                     const unsigned buffer = buffers + slot * kPairBufferBytes;
                     const unsigned full = map_to_rank(shared_address(&control.full[slot]), 0);
@@ -318,11 +324,11 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
             unsigned phase = 0, drained_phase = 1;
             bool ok = true;
             for (unsigned t = pair; ok && t < tiles; t += pairs) {
-                if (!wait_barrier(&control.drained, drained_phase, &control.abort)) break;
+                if (!wait_warp(&control.drained, drained_phase, &control.abort)) break;
                 drained_phase ^= 1u;
                 fence_after();
                 for (int stage = 0; stage < stages; ++stage) {
-                    if (!wait_barrier(&control.full[slot], phase, &control.abort)) { ok = false; break; }
+                    if (!wait_warp(&control.full[slot], phase, &control.abort)) { ok = false; break; }
                     fence_after();
                     if (elect_one()) {
                         const unsigned buffer = buffers + slot * kPairBufferBytes;
@@ -372,7 +378,7 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
 #pragma unroll
                 for (int c = 0; c < kWriterColumns; c += 32) bias[c + lane] = column0 + c + lane < p.n ? load1(p.bias, p.bias_dt, column0 + c + lane) : 0.0f;
             }
-            if (!__all_sync(0xffffffffu, wait_barrier(&control.done, phase, &control.abort))) break;
+            if (!wait_warp(&control.done, phase, &control.abort)) break;
             phase ^= 1u;
             fence_after();
             float v[kWriterColumns];
@@ -497,7 +503,7 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
         int slot = 0;
         unsigned phase = 1;
         for (int stage = first; stage < last; ++stage) {
-            if (!wait_barrier(&control.empty[slot], phase, &control.abort)) break;
+            if (!wait_warp(&control.empty[slot], phase, &control.abort)) break;
             if (elect_one()) {
                 const unsigned buffer = buffers + slot * buffer_bytes, full = shared_address(&control.full[slot]);
                 mbarrier_expect_bytes(&control.full[slot], kCodeBytes + a_bytes + 2 * kTiles * 512);
@@ -549,7 +555,7 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
     __align__(16) float bias[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) bias[e] = p.bias && n0 + e < p.n ? load1(p.bias, p.bias_dt, n0 + e) : 0.0f;
-    if (warp >= 2 && __all_sync(0xffffffffu, wait_barrier(&control.done, 0, &control.abort))) {
+    if (warp >= 2 && wait_warp(&control.done, 0, &control.abort)) {
         // all copies into the ring and all products out of it are over: its memory takes the accumulator, 128 floats a column
         fence_after();
         const unsigned mine = buffers + ((warp & 3) * 32 + lane) * 4;       // the tensor-memory lane is the row of b
