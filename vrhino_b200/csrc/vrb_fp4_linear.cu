@@ -317,6 +317,11 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
                 if (++slot == kPairStages) { slot = 0; phase ^= 1u; }
             }
         }
+        // the last products' arrivals on the barriers of empty buffers: none may be under way when the CTA ends
+        for (int left = kPairStages; ok && left > 0; --left) {
+            ok = wait_warp(&control.empty[slot], phase, &control.abort);
+            if (++slot == kPairStages) { slot = 0; phase ^= 1u; }
+        }
     } else if (warp == 1) {
         if (rank == 0) {
             constexpr uint32_t instruction = instruction_descriptor<FORMAT>(kPairTile, kPairTile);
@@ -502,8 +507,9 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
     if (warp == 0) {
         int slot = 0;
         unsigned phase = 1;
+        bool ok = true;
         for (int stage = first; stage < last; ++stage) {
-            if (!wait_warp(&control.empty[slot], phase, &control.abort)) break;
+            if (!wait_warp(&control.empty[slot], phase, &control.abort)) { ok = false; break; }
             if (elect_one()) {
                 const unsigned buffer = buffers + slot * buffer_bytes, full = shared_address(&control.full[slot]);
                 mbarrier_expect_bytes(&control.full[slot], kCodeBytes + a_bytes + 2 * kTiles * 512);
@@ -513,6 +519,10 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
                 load_own_box(buffer + kCodeBytes + 2 * kScaleBytes, &a_map, stage * kStageBytes, static_cast<int>(a0), full);
             }
             __syncwarp();
+            if (++slot == q.ring) { slot = 0; phase ^= 1u; }
+        }
+        for (int left = q.ring; ok && left > 0; --left) {   // as in the pair kernel
+            ok = wait_warp(&control.empty[slot], phase, &control.abort);
             if (++slot == q.ring) { slot = 0; phase ^= 1u; }
         }
     } else if (warp == 1) {
