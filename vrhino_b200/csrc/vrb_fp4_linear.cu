@@ -187,9 +187,9 @@ __device__ __forceinline__ void tile_of(unsigned index, unsigned row_tiles, unsi
     row_tile = first + within - column_tile * height;
 }
 
-// ACT: 0 none, 1 SiLU, 2 GELU-tanh, 3 any other kind.  v[0 .. N) = act(alpha * v + bias); without an activation the product
-// is rounded to F32 before the bias is added, so that the result has the bits of vrb_linear_output on the stored
-// accumulation.  bias: F32 in shared memory or nullptr.
+// ACT: 0 none, 1 SiLU and 2 GELU-tanh for bf16 results, 3 any other kind, 4 and 5 as 1 and 2 for F32 results.  v[0 .. N) =
+// act(alpha * v + bias); without an activation the product is rounded to F32 before the bias is added, so that the result has the
+// bits of vrb_linear_output on the stored accumulation.  bias: F32 in shared memory or nullptr.
 template <int ACT, int N>
 __device__ __forceinline__ void finish_columns(float* v, const float* bias, float alpha, int kind) {
 #pragma unroll
@@ -197,22 +197,24 @@ __device__ __forceinline__ void finish_columns(float* v, const float* bias, floa
         float4 b = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (bias) b = *reinterpret_cast<const float4*>(bias + i);
         unsigned long long lo, hi;
-        if constexpr (ACT == 1 || ACT == 2) {
-            lo = fma_f32x2(pack_f32x2(v[i], v[i + 1]), pack_f32x2(alpha, alpha), pack_f32x2(b.x, b.y));
-            hi = fma_f32x2(pack_f32x2(v[i + 2], v[i + 3]), pack_f32x2(alpha, alpha), pack_f32x2(b.z, b.w));
-        } else {
+        if constexpr (ACT == 0 || ACT == 3) {
             lo = add_f32x2(pack_f32x2(__fmul_rn(v[i], alpha), __fmul_rn(v[i + 1], alpha)), pack_f32x2(b.x, b.y));
             hi = add_f32x2(pack_f32x2(__fmul_rn(v[i + 2], alpha), __fmul_rn(v[i + 3], alpha)), pack_f32x2(b.z, b.w));
+        } else {
+            lo = fma_f32x2(pack_f32x2(v[i], v[i + 1]), pack_f32x2(alpha, alpha), pack_f32x2(b.x, b.y));
+            hi = fma_f32x2(pack_f32x2(v[i + 2], v[i + 3]), pack_f32x2(alpha, alpha), pack_f32x2(b.z, b.w));
         }
         if constexpr (ACT == 1 || ACT == 2) {
-            gate_pair<ACT>(lo, v[i], v[i + 1]);
-            gate_pair<ACT>(hi, v[i + 2], v[i + 3]);
+            gate_pair<ACT, true>(lo, v[i], v[i + 1]);
+            gate_pair<ACT, true>(hi, v[i + 2], v[i + 3]);
         } else {
             unpack_f32x2(lo, v[i], v[i + 1]);
             unpack_f32x2(hi, v[i + 2], v[i + 3]);
-            if constexpr (ACT == 3)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[i + e] = activation_value(kind, v[i + e]);
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (ACT == 3) v[i + e] = activation_value(kind, v[i + e]);
+                if constexpr (ACT > 3) v[i + e] = gate_value<ACT - 3>(v[i + e]);
+            }
         }
     }
 }
@@ -749,16 +751,17 @@ int launch_split(const LinearMaps& maps, const LinearArgs& p, const LinearPlan& 
 template <int FORMAT>
 int launch_split(const LinearMaps& maps, const LinearArgs& p, const LinearPlan& plan, cudaStream_t s) {
     if (p.activation == VRB_NO_ACTIVATION) return launch_split<FORMAT, 0>(maps, p, plan, s);
-    if (p.activation == VRB_SILU) return launch_split<FORMAT, 1>(maps, p, plan, s);
-    if (p.activation == VRB_GELU_TANH) return launch_split<FORMAT, 2>(maps, p, plan, s);
+    const bool f32 = p.out_dt == VRB_F32;
+    if (p.activation == VRB_SILU) return f32 ? launch_split<FORMAT, 4>(maps, p, plan, s) : launch_split<FORMAT, 1>(maps, p, plan, s);
+    if (p.activation == VRB_GELU_TANH) return f32 ? launch_split<FORMAT, 5>(maps, p, plan, s) : launch_split<FORMAT, 2>(maps, p, plan, s);
     return launch_split<FORMAT, 3>(maps, p, plan, s);
 }
 
 template <int FORMAT, int OUT>
 int launch_linear(const LinearMaps& maps, const LinearArgs& p, cudaStream_t s) {
     if (p.activation == VRB_NO_ACTIVATION) return launch_pair<FORMAT, 0, OUT>(maps, p, s);
-    if (p.activation == VRB_SILU) return launch_pair<FORMAT, 1, OUT>(maps, p, s);
-    if (p.activation == VRB_GELU_TANH) return launch_pair<FORMAT, 2, OUT>(maps, p, s);
+    if (p.activation == VRB_SILU) return launch_pair<FORMAT, OUT == VRB_F32 ? 4 : 1, OUT>(maps, p, s);
+    if (p.activation == VRB_GELU_TANH) return launch_pair<FORMAT, OUT == VRB_F32 ? 5 : 2, OUT>(maps, p, s);
     return launch_pair<FORMAT, 3, OUT>(maps, p, s);
 }
 

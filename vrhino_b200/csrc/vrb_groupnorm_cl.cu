@@ -94,19 +94,22 @@ __device__ __forceinline__ void store_vec(float* p, const float (&v)[V]) {
     else __stcs(p, v[0]);
 }
 
-// act((v - mean) scale + shift) of a thread's V channels: F32 values that are rounded once afterwards.  SiLU and GELU-tanh by
-// pairs (gate_pair: three special functions for two values; with four the normalise pass of 25 MB waits for that unit).  ACT 3:
-// any other kind.
+// act((v - mean) scale + shift) of a thread's V channels: F32 values that are rounded once afterwards.  SiLU and GELU-tanh in
+// bf16 by pairs (gate_pair: three special functions for two values; with four the normalise pass of 25 MB waits for that unit), in
+// F32, twice the bytes a value, one by one to F32's accuracy.  ACT 3: any other kind.
 template <int ACT, typename T, int V>
 __device__ __forceinline__ void normalise(const Vec<T, V>& v, const float (&mean)[V], const float (&scale)[V], const float (&shift)[V], int kind, float (&y)[V]) {
 #pragma unroll
     for (int e = 0; e < V; ++e) y[e] = fmaf(v.get(e) - mean[e], scale[e], shift[e]);
-    if constexpr (ACT == 1 || ACT == 2) {
+    if constexpr ((ACT == 1 || ACT == 2) && sizeof(T) == 4) {
 #pragma unroll
-        for (int e = 0; e + 1 < V; e += 2) gate_pair<ACT>(pack_f32x2(y[e], y[e + 1]), y[e], y[e + 1]);
+        for (int e = 0; e < V; ++e) y[e] = gate_value<ACT>(y[e]);
+    } else if constexpr (ACT == 1 || ACT == 2) {
+#pragma unroll
+        for (int e = 0; e + 1 < V; e += 2) gate_pair<ACT, false>(pack_f32x2(y[e], y[e + 1]), y[e], y[e + 1]);
         if constexpr (V == 1) {
             float unused;
-            gate_pair<ACT>(pack_f32x2(y[0], 0.0f), y[0], unused);
+            gate_pair<ACT, false>(pack_f32x2(y[0], 0.0f), y[0], unused);
         }
     } else if constexpr (ACT == 3) {
 #pragma unroll
