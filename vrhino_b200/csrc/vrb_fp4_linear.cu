@@ -218,6 +218,17 @@ __device__ __forceinline__ void finish_columns(float* v, const float* bias, floa
         }
     }
 }
+// The product of the tensor scales as two factors: accumulations take `before` (1 as a rule) ahead of `alpha`.  Where the product
+// leaves F32's normal range, as that of two ordinary scales can, the larger scale comes first: what it makes overflow the smaller
+// one, above 1 then, does not bring back, and only the last product falls below the normal range.
+struct Scale {
+    float before, alpha;
+};
+__device__ __forceinline__ Scale tensor_scale(const float* a, const float* b) {
+    const float ga = a ? *a : 1.0f, gb = b ? *b : 1.0f, product = __fmul_rn(ga, gb);
+    if ((product < 1.17549435e-38f || product > 3.402823466e38f) && ga != 0.0f && gb != 0.0f) return {fmaxf(ga, gb), fminf(ga, gb)};
+    return {1.0f, product};
+}
 // 64 bytes of this lane's row into the warp's box of 32 rows (64-byte swizzle: 16-byte pieces by bits 1-2 of the row)
 __device__ __forceinline__ void stage_row(unsigned box, int lane, const uint32_t (&w)[16]) {
 #pragma unroll
@@ -370,7 +381,7 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
     } else {
         const int quarter = warp & 3;                  // the 32 tensor-memory lanes this warp may read
         const int writer = warp - 2, group = writer >> 2;   // its 64 of the columns
-        const float alpha = __fmul_rn(p.a_scale ? *p.a_scale : 1.0f, p.b_scale ? *p.b_scale : 1.0f);
+        const Scale scale = tensor_scale(p.a_scale, p.b_scale);
         const unsigned box = shared_address(shared.boxes[writer]);
         float* scratch = reinterpret_cast<float*>(shared.boxes[writer]);
         float* bias = shared.bias[writer];
@@ -396,12 +407,15 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
             fence_before();
             __syncwarp();
             if (lane == 0) arrive_cluster(drained);
+            if (scale.before != 1.0f)
+#pragma unroll
+                for (int c = 0; c < kWriterColumns; ++c) v[c] *= scale.before;
             const int64_t row0 = static_cast<int64_t>(row_tile) * kPairTile + rank * kRows + quarter * 32;
             if (p.boxed) {
                 constexpr int N = OUT == VRB_BF16 ? 32 : 16;   // columns of a box
 #pragma unroll
                 for (int c = 0; c < kWriterColumns; c += N) {
-                    finish_columns<ACT, N>(v + c, p.bias ? bias + c : nullptr, alpha, p.activation);
+                    finish_columns<ACT, N>(v + c, p.bias ? bias + c : nullptr, scale.alpha, p.activation);
                     uint32_t w[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) w[i] = OUT == VRB_BF16 ? pack_bf16x2(v[c + 2 * i % N], v[c + (2 * i + 1) % N]) : __float_as_uint(v[c + i % N]);
@@ -418,7 +432,7 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
                 const int height = static_cast<int>(p.m - row0 < 32 ? p.m - row0 : 32);
 #pragma unroll
                 for (int c = 0; c < kWriterColumns; c += 16) {
-                    finish_columns<ACT, 16>(v + c, p.bias ? bias + c : nullptr, alpha, p.activation);
+                    finish_columns<ACT, 16>(v + c, p.bias ? bias + c : nullptr, scale.alpha, p.activation);
                     __syncwarp();
 #pragma unroll
                     for (int i = 0; i < 16; ++i) scratch[lane * 16 + (i ^ (lane >> 1 & 15))] = v[c + i];
@@ -563,7 +577,7 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
     }
     const int height = static_cast<int>(p.m - a0 < q.columns ? p.m - a0 : q.columns);
     const int64_t n0 = b0 + lane * 4;                  // the four rows of b that this thread finishes
-    const float alpha = __fmul_rn(p.a_scale ? *p.a_scale : 1.0f, p.b_scale ? *p.b_scale : 1.0f);
+    const Scale scale = tensor_scale(p.a_scale, p.b_scale);
     __align__(16) float bias[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) bias[e] = p.bias && n0 + e < p.n ? load1(p.bias, p.bias_dt, n0 + e) : 0.0f;
@@ -608,7 +622,10 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
             int64_t at = (a0 + c) * p.n + n0;
 #pragma unroll
             for (int i = 0; i < 4; ++i, at += p.n) {
-                finish_columns<ACT, 4>(y[i], bias, alpha, p.activation);
+                if (scale.before != 1.0f)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[i][e] *= scale.before;
+                finish_columns<ACT, 4>(y[i], bias, scale.alpha, p.activation);
                 if (c + i >= end) break;
                 if (p.quads && p.out_dt == VRB_BF16) {
                     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(pack_bf16x2(y[i][0], y[i][1]), pack_bf16x2(y[i][2], y[i][3]));
