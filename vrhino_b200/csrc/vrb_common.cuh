@@ -8,6 +8,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <utility>
 
 #include "vrb.h"
 
@@ -57,27 +58,37 @@ inline int after_launch(const char* what) {
 // Without the attribute pdl_wait() returns at once.
 extern std::atomic<int> g_launch_overlap;
 
+// A launch with overlap, in clusters of `cluster` CTAs along x (0: what the kernel itself says).
 template <typename... KArgs, typename... Args>
-inline void launch_overlapped(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {
+inline void launch_clusters(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t stream, Args&&... args) {
     cudaLaunchConfig_t config = {};
     config.gridDim = grid;
     config.blockDim = block;
     config.dynamicSmemBytes = smem;
     config.stream = stream;
-    cudaLaunchAttribute attribute[1];
-    if (g_launch_overlap.load(std::memory_order_relaxed) != 0) {
-        attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attribute[0].val.programmaticStreamSerializationAllowed = 1;
-        config.attrs = attribute;
+    cudaLaunchAttribute attributes[2];
+    config.attrs = attributes;
+    if (cluster > 0) {
+        attributes[0].id = cudaLaunchAttributeClusterDimension;
+        attributes[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+        attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
         config.numAttrs = 1;
+    }
+    if (g_launch_overlap.load(std::memory_order_relaxed) != 0) {
+        cudaLaunchAttribute& attribute = attributes[config.numAttrs++];
+        attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attribute.val.programmaticStreamSerializationAllowed = 1;
         if (cudaLaunchKernelEx(&config, kernel, static_cast<KArgs>(args)...) == cudaSuccess) return;
         // a driver / stream that refuses the attribute: plain launches from here on
         cudaGetLastError();
         g_launch_overlap.store(0, std::memory_order_relaxed);
-        config.attrs = nullptr;
-        config.numAttrs = 0;
+        --config.numAttrs;
     }
     cudaLaunchKernelEx(&config, kernel, static_cast<KArgs>(args)...);   // an error stays for after_launch()
+}
+template <typename... KArgs, typename... Args>
+inline void launch_overlapped(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {
+    launch_clusters(kernel, grid, block, smem, 0, stream, std::forward<Args>(args)...);
 }
 
 // Persistent-style grid: enough CTAs to fill every SM `per_sm` times, never more than `work`.

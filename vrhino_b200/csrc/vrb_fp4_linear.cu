@@ -748,20 +748,8 @@ int launch_split(const LinearMaps& maps, const LinearArgs& p, const LinearPlan& 
     static std::atomic<uint64_t> allowed{0};
     if (int rc = allow_shared(fp4_linear_split_kernel<FORMAT, ACT>, kSplitMostShared, allowed, "fp4_linear")) return rc;
     const int64_t tiles = ((p.m + q.columns - 1) / q.columns) * ((p.n + kRows - 1) / kRows);
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(static_cast<unsigned>(tiles * q.splits));
-    config.blockDim = dim3(kSplitThreads);
-    config.dynamicSmemBytes = bytes;
-    config.stream = s;
-    cudaLaunchAttribute attributes[2];
-    attributes[0].id = cudaLaunchAttributeClusterDimension;
-    attributes[0].val.clusterDim.x = static_cast<unsigned>(q.splits);
-    attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
-    attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attributes[1].val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = attributes;
-    config.numAttrs = g_launch_overlap.load(std::memory_order_relaxed) != 0 ? 2 : 1;
-    cudaLaunchKernelEx(&config, fp4_linear_split_kernel<FORMAT, ACT>, maps.a, maps.b, maps.a_scales, maps.b_scales, q);   // an error stays for after_launch()
+    launch_clusters(fp4_linear_split_kernel<FORMAT, ACT>, dim3(static_cast<unsigned>(tiles * q.splits)), dim3(kSplitThreads), bytes, q.splits, s, maps.a, maps.b, maps.a_scales,
+                    maps.b_scales, q);
     return after_launch("fp4_linear");
 }
 

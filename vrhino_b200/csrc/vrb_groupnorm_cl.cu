@@ -704,24 +704,6 @@ size_t workspace_size(const GclGeom& g) {
     return partial_bytes(g) + (g.groups > kInlineGroups ? up256(static_cast<size_t>(g.batch) * g.groups * sizeof(float2)) : 0);
 }
 
-template <typename... KArgs, typename... Args>
-void launch_clusters(void (*kernel)(KArgs...), unsigned ctas, int threads, size_t shared, int cluster, cudaStream_t stream, Args&&... args) {
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(ctas);
-    config.blockDim = dim3(static_cast<unsigned>(threads));
-    config.dynamicSmemBytes = shared;
-    config.stream = stream;
-    cudaLaunchAttribute attributes[2];
-    attributes[0].id = cudaLaunchAttributeClusterDimension;
-    attributes[0].val.clusterDim.x = static_cast<unsigned>(cluster);
-    attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
-    attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attributes[1].val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = attributes;
-    config.numAttrs = g_launch_overlap.load(std::memory_order_relaxed) != 0 ? 2 : 1;
-    cudaLaunchKernelEx(&config, kernel, static_cast<KArgs>(args)...);   // an error stays for after_launch()
-}
-
 struct GclCall {
     const void *x, *weight, *bias;
     void* out;
@@ -732,7 +714,7 @@ struct GclCall {
 template <typename T, int V, int E, int ACT>
 int run_cluster(const GclCall& c, const GclGeom& g, cudaStream_t s) {
     const int64_t units = g.batch * ((g.vectors + g.slab - 1) / g.slab);
-    launch_clusters(gcl_cluster_kernel<T, V, E, ACT>, static_cast<unsigned>(units * g.cluster), kClusterThreads, 0, g.cluster, s, static_cast<const T*>(c.x), c.weight, c.w_dt, c.bias,
+    launch_clusters(gcl_cluster_kernel<T, V, E, ACT>, dim3(static_cast<unsigned>(units * g.cluster)), dim3(kClusterThreads), 0, g.cluster, s, static_cast<const T*>(c.x), c.weight, c.w_dt, c.bias,
                     c.b_dt, static_cast<T*>(c.out), g, c.eps, c.activation);
     return after_launch("group_norm_channels_last");
 }
@@ -748,7 +730,7 @@ template <typename T, int E, int ACT>
 int run_resident(const GclCall& c, const GclGeom& g, cudaStream_t s) {
     static std::atomic<uint64_t> allowed{0};
     if (int rc = allow_shared(gcl_resident_kernel<T, E, ACT>, resident_most(static_cast<int>(16 / sizeof(T)) / E), allowed, "group_norm_channels_last")) return rc;
-    launch_clusters(gcl_resident_kernel<T, E, ACT>, static_cast<unsigned>(g.batch * (g.vectors / g.slab) * g.cluster), kResidentThreads, resident_bytes(g), g.cluster, s,
+    launch_clusters(gcl_resident_kernel<T, E, ACT>, dim3(static_cast<unsigned>(g.batch * (g.vectors / g.slab) * g.cluster)), dim3(kResidentThreads), resident_bytes(g), g.cluster, s,
                     static_cast<const T*>(c.x), c.weight, c.w_dt, c.bias, c.b_dt, static_cast<T*>(c.out), g, c.eps, c.activation);
     return after_launch("group_norm_channels_last");
 }
