@@ -333,8 +333,11 @@ int vrb_group_norm_apply_scatter(const void* x, int dtype, const void* weight, i
  * back.  Unlike vrb_group_norm + SiLU the normalised value is not rounded before the activation.
  * activation: a vrb_activation_kind or VRB_NO_ACTIVATION.  weight / bias (F32 or BF16, [channels]) may be
  * NULL and are used as stored.  out may be x.  Results do not depend on the launch's timing.
- * workspace: vrb_group_norm_channels_last_workspace_bytes() bytes of device scratch, 256-byte aligned
- * (0 bytes: NULL is accepted); calls that may overlap on the GPU need scratch of their own. */
+ * The variance is an F32: squares of distances from the mean have to lie within its range, as in vrb_group_norm.
+ * VRB_SILU and VRB_GELU_TANH are y sigmoid(w), exact to the result's type relative to their value (F32: 2^-21, GELU-tanh
+ * 2^-22 |w| more; BF16: rounded once, a sigmoid below 2^-126 is 0); -infinity gives NaN, as in vrb_activation.
+ * workspace: vrb_group_norm_channels_last_workspace_bytes() bytes of device scratch, 256-byte aligned, enough at
+ * any alignment of x and out (0 bytes: NULL is accepted); calls that may overlap on the GPU need scratch of their own. */
 #define VRB_NO_ACTIVATION (-1)
 size_t vrb_group_norm_channels_last_workspace_bytes(int dtype, int64_t batch, int64_t spatial, int64_t channels, int groups);
 int vrb_group_norm_channels_last(const void* x, int dtype, const void* weight, int weight_dtype,
@@ -353,7 +356,7 @@ int vrb_group_norm_channels_last(const void* x, int dtype, const void* weight, i
  *   scales  vrb_fp4_scale_bytes(format, rows, k) bytes, 16-byte aligned, in the order the tensor core takes
  *           them: tiles of 128 rows x 4 blocks of 512 bytes, block tiles innermost; the scale of (row, block) is byte
  *           ((row / 128) * ceil(blocks / 4) + block / 4) * 512 + (row % 32) * 16 + (row % 128) / 32 * 4 + block % 4;
- *           padding bytes are zero
+ *           padding bytes are zero, e4m3 scales have no sign
  * Weights are packed once and kept; activations are packed per call.  The reference stores weights in 8 bits or as
  * integers (QuantType, native/include/vrhino/tensor.h:35) and has no 4-bit floating point. */
 typedef enum vrb_fp4_format { VRB_NVFP4 = 0, VRB_MXFP4 = 1 } vrb_fp4_format;
@@ -367,6 +370,7 @@ int vrb_fp4_tensor_scale(const void* x, int dtype, int64_t count, float* tensor_
 /* Packs x [rows, k].  NVFP4: scale = e4m3(min(amax / (6 tensor_scale), 448)), element = e2m1(x / (tensor_scale *
  * scale)); MXFP4: scale = 2^max(floor(log2 amax) - 2, -127), element = e2m1(x / scale), with amax the block's
  * largest magnitude.  Both roundings are those of the exact quotients: to nearest, ties to the even code, saturating.
+ * rows and k are positive here and in all calls that follow.
  * tensor_scale: one F32 on the device (NULL = 1), finite and >= 0.  A block that holds an infinity or a NaN (or
  * meets a tensor scale that is one) gets the NaN scale (0x7f / 0xff) and zero elements. */
 int vrb_fp4_quantize(int format, const void* x, int dtype, const float* tensor_scale, void* codes, void* scales,
@@ -378,8 +382,9 @@ int vrb_fp4_dequantize(int format, const void* codes, const void* scales, const 
 
 /* The linear over two packed operands of one format, on the tensor cores that multiply block-scaled 4-bit elements:
  *   out[m, n] = act(a_tensor_scale * b_tensor_scale * sum_k a[m, k] b[n, k] + bias[n])      [rows_a, rows_b]
- * accumulated in F32, one rounding to out_dtype.  bias (F32 or BF16, [rows_b]) may be NULL; activation: a
- * vrb_activation_kind or VRB_NO_ACTIVATION.  With F32 output, no bias and no activation the result is the accumulation
+ * accumulated in F32, one rounding to out_dtype; the tensor scales are applied one after the other where their product
+ * leaves F32's normal range.  bias (F32 or BF16, [rows_b]) may be NULL; activation: a vrb_activation_kind or
+ * VRB_NO_ACTIVATION, as exact as in vrb_group_norm_channels_last.  With F32 output, no bias and no activation the result is the accumulation
  * that vrb_linear_output and its merged forms read.  Replaces a dequantisation (vrb_dequantize) and CudaBackend::linear
  * (:3661-3866) where the weight is kept in 4 bits.  Needs the driver's cuTensorMapEncodeTiled (VRB_ERR_UNSUPPORTED
  * otherwise).  Every wait inside is bounded; vrb_async_wait_failures reports one that ran out. */

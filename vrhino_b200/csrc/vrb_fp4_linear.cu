@@ -694,7 +694,8 @@ int launch_pair(const LinearMaps& maps, const LinearArgs& p, cudaStream_t s) {
 }
 // Which kernel, and the split kernel's tile and cluster: the least of the times that a model gives, in nanoseconds, fitted to
 // both kernels on B200 (back to back in a graph; the choice is within 3 % of the best on 24 shapes from 1 x 512 x 512
-// to 4000 x 6000 and to k past 30000).  Pair kernel: 4300 + 500 a tile + 290 a stage.  Split kernel: 2300 + 19 a column
+// to 4000 x 6000 and to k past 30000), with operands that L2 held: a weight that comes from HBM takes longer a stage (18 KB a CTA in
+// 265 ns are 10 TB/s over the SMs), and the choice of clusters for it is not measured.  Pair kernel: 4300 + 500 a tile + 290 a stage.  Split kernel: 2300 + 19 a column
 // of the tile + 265 a stage, and 800 + 130 a CTA to meet in a cluster; one CTA to an SM, what does not fit at once takes turns.
 struct LinearPlan {
     int columns;   // 0: pair kernel

@@ -636,7 +636,9 @@ void set_width(GclGeom& g, int v) {
     g.rpp = kThreads / g.slab;
     if (g.rpp > all_rows(g)) g.rpp = static_cast<int>(all_rows(g));
 }
-// CTAs of the statistics pass per batch entry: one per SM over the whole batch, no more than passes over the rows
+// CTAs of the statistics pass per batch entry: one per SM over the whole batch, no more than passes over the rows.  Rounded up, here
+// and in the normalise pass: batches that divide the SMs unevenly start a few CTAs more than there are SMs, which run after the rest
+// (1433600 rows of 256 channels, bf16 with SiLU: 362 us in 1, 2 or 4 entries, 540 to 586 in 3, 5, 8, 16 or 28).
 void set_splits(GclGeom& g) {
     const int64_t want = (sm_count() + g.batch - 1) / g.batch, most = (all_rows(g) + g.rpp - 1) / g.rpp;
     g.splits = static_cast<int>(want < most ? want : most);
@@ -644,7 +646,7 @@ void set_splits(GclGeom& g) {
 // The slab and cluster of gcl_cluster, or false: the slab is the least run of whole groups and whole vectors of 64 bytes or
 // more (a row's piece of a slab should fill memory sectors), its rows have to fit kMostRows rows of a thread in up to eight
 // CTAs, and all clusters should be at work at once.  Measured against the passes (bf16 with SiLU, back to back): 64 rows of 512
-// channels 4.9 us against 8.8, 256 rows 5.7 against 9.2, 2048 rows 8.0 against 11.8; with 16 rows a thread the code of a
+// channels 3.5 us against 10.1, 256 rows 4.1 against 10.6, 2048 rows 5.5 against 11.1; with 16 rows a thread the code of a
 // once-run kernel costs more than a second read of x (4096 rows 15.9 against 12.6).
 bool set_cluster(GclGeom& g, int v, int element) {
     int groups = 1;
@@ -663,11 +665,11 @@ bool set_cluster(GclGeom& g, int v, int element) {
 // The slab and cluster of gcl_resident, or false: slabs of whole groups and of 16-byte vectors (whose channels lie in one group or
 // two by two), at least 64 bytes or else 32 of every row, whose rows fit the shared memory of up to eight CTAs; all clusters at work
 // at once, a CTA to an SM, on half of the SMs or else a quarter (`room`: CTAs that fit for clusters of 1 to 8; a second wave costs
-// as much as the first).  Measured against the passes (bf16 with SiLU, back to back): 2400 rows of 512 channels 6.8 us against 11.6,
-// 8000 rows 10.3 against 13.1, 16000 rows 15.1 against 16.4; 4 x 4096 rows 12.7 against 16.1; 8 x 4096 rows of 320 channels 17.3
-// against 34.1.  Pieces of 32 bytes come at half the rate: 20000 rows of 512 channels, 20 of a thread, 17.9 against 18.8, 24960 rows
-// 20.4 against 20.1, so those end at 20 rows.  On a quarter of the SMs: 3000 rows of 192 channels, 3 of a thread, 7.1 against 9.6,
-// 16384 of 128, 8 of a thread, 10.1 against 10.9, 9216 of 320, 12 of a thread, 12.7 against 12.3.
+// as much as the first).  Measured against the passes (bf16 with SiLU, back to back): 2400 rows of 512 channels 6.9 us against 11.5,
+// 8000 rows 10.6 against 13.1, 16000 rows 15.2 against 15.8; 4 x 4096 rows 12.9 against 15.5; 8 x 4096 rows of 320 channels 17.6
+// against 30.1.  Pieces of 32 bytes come at half the rate: 20000 rows of 512 channels, 20 of a thread, 16.5 against 17.9, 24960 rows
+// 20.4 against 20.1, so those end at 20 rows.  On a quarter of the SMs: 3000 rows of 192 channels, 3 of a thread, 7.8 against 11.1,
+// 16384 of 128, 8 of a thread, 10.6 against 12.0, 9216 of 320, 12 of a thread, 12.7 against 12.3.
 bool set_resident(GclGeom& g, int v, int element, const int* room) {
     const int entries = v / entry_channels(g, v);
     if (v * element != 16 || entries > 4 || (entries > 2 && element == 4) || g.spatial > INT32_MAX) return false;

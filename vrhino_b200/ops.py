@@ -672,7 +672,8 @@ class B200Backend:
 
     def fp4_quantize(self, raw, format=NVFP4, tensor_scale=None, out=None):
         """Packs x [..., k] into 4 bits an element with a scale per block of a row; NVFP4 takes a device F32 tensor scale
-        (fp4_tensor_scale, or one calibrated beforehand; None = 1)."""
+        (fp4_tensor_scale, or one calibrated beforehand; None = 1).  Rows and k have to be positive: an empty batch has no
+        packed form."""
         dtype = self._dtype_of(raw)
         x = _dense(self.copy_to_device(raw, dtype))
         count, device = x.numel(), x.device
