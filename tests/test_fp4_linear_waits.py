@@ -102,3 +102,22 @@ def test_copying_warps_outwait_the_products():
     loops = re.findall(r"for \(int left = (\w+(?:\.\w+)?); ok && left > 0; --left\) \{\s*ok = wait_warp\(&control\.empty\[slot\], phase, &control\.abort\);"
                        r"\s*if \(\+\+slot == (\w+(?:\.\w+)?)\) \{ slot = 0; phase \^= 1u; \}\s*\}", text)
     assert loops == [("kPairStages", "kPairStages"), ("q.ring", "q.ring")]
+
+
+def test_tensor_memory_goes_back_before_a_cluster_meets():
+    """An allocation of tensor memory waits until the SM has enough of it, and other libraries' kernels take it too.  A CTA of the
+    split kernel that held its part while it waited for its cluster, and a pair of such a kernel's CTAs that waits for each other
+    likewise, could each hold what the other needs.  So the split kernel allocates, works alone, gives back, and only then meets
+    its cluster; the pair kernel, whose CTAs meet before that, leaves no shared memory for another kernel on its SMs."""
+    text = _text()
+    split = text[text.index("fp4_linear_split_kernel(const __grid_constant__"):]
+    split = split[:split.index("\n}\n")]
+    assert split.count("tcgen05.alloc") == 1 and split.count("tcgen05.dealloc") == 1
+    held = split[split.index("tcgen05.alloc"):split.index("tcgen05.dealloc")]
+    assert "cluster_sync" not in held and "barrier.cluster" not in held
+    assert "wait_reads()" in held and "__syncthreads();" in held[held.index("wait_reads()"):]
+    assert split.count("cluster_sync();") == 2
+    pair = re.search(r"static_assert\(sizeof\(PairShared\) <= (\d+) \* 1024", text)
+    stages, threads = (int(re.search(rf"constexpr int {name} = (\d+);", text).group(1)) for name in ("kPairStages", "kPairThreads"))
+    buffers = stages * (2 * 128 * 128 + 3 * 2048) + 16 * 32 * 64 + 16 * 64 * 4
+    assert pair and threads == 576 and 228 * 1024 - 1024 - buffers < 2 * 1024      # what another CTA could have beside it

@@ -83,6 +83,11 @@ __device__ __forceinline__ bool wait_barrier(uint64_t* barrier, unsigned parity,
 __device__ __forceinline__ bool wait_warp(uint64_t* barrier, unsigned parity, volatile int* abort) {
     return __all_sync(0xffffffffu, wait_barrier(barrier, parity, abort));
 }
+// After a wait that gave up: lets copies and products in flight end before their memory goes
+__device__ __noinline__ void let_end() {
+    const unsigned long long start = now_ns();
+    for (int i = 0; i < 100000 && now_ns() - start < 20000000ull; ++i) __nanosleep(1000);
+}
 __device__ __forceinline__ unsigned cluster_rank() {
     unsigned r;
     asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
@@ -448,10 +453,7 @@ fp4_linear_pair_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_c
     __syncwarp();
     fence_before();
     __syncthreads();
-    if (control.abort) {   // let copies and products in flight end before their memory goes
-        const unsigned long long start = now_ns();
-        for (int i = 0; i < 100000 && now_ns() - start < 20000000ull; ++i) __nanosleep(1000);
-    }
+    if (control.abort) let_end();
     cluster_sync();        // the other CTA's products and arrivals reach into this one
     fence_after();
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(kPairColumns));
@@ -593,8 +595,15 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
             for (int i = 0; i < 16; ++i) asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + (c + i) * 512), "f"(v[i]) : "memory");
         }
     }
+    // Tensor memory goes back before the cluster meets: a CTA that held it while it waited for the others could wait for good, where
+    // one of those waits for the tensor memory of another kernel's cluster, which waits for this CTA's.
     __syncwarp();
-    if (q.splits > 1) cluster_sync(); else __syncthreads();
+    fence_before();
+    __syncthreads();
+    if (control.abort) let_end();
+    fence_after();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(q.tensor_columns));
+    if (q.splits > 1) cluster_sync();
     // this CTA's share of the columns, four columns x four rows of b to a thread: a warp writes 128 consecutive elements of four
     // rows of the result, and the loads of four columns from four CTAs are in flight together
     const int share = (height + q.splits * 4 - 1) / (q.splits * 4) * 4, begin = rank * share, end = min(height, begin + share);
@@ -641,15 +650,6 @@ fp4_linear_split_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_
     }
     __syncwarp();
     if (q.splits > 1) cluster_sync();   // no CTA's memory goes while another reads it
-    __syncwarp();
-    fence_before();
-    __syncthreads();
-    if (control.abort) {       // let copies and products in flight end before their memory goes
-        const unsigned long long start = now_ns();
-        for (int i = 0; i < 100000 && now_ns() - start < 20000000ull; ++i) __nanosleep(1000);
-    }
-    fence_after();
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(q.tensor_columns));
 }
 
 // ----------------------------------------------------------------------------------------- host side --
@@ -737,7 +737,7 @@ int launch_split(const LinearMaps& maps, const LinearArgs& p, const LinearPlan& 
     bytes += 1024;
     // A CTA takes at least the share of an SM's shared memory that it takes of the tensor memory (as the pair kernel does, with
     // all of both).  So whatever CTAs of these kernels share an SM, from one launch or several streams, no tensor memory
-    // allocation ever waits: two clusters that waited for each other's CTAs would wait for good.
+    // allocation ever waits for another CTA of these kernels.
     q.tensor_columns = 32;
     while (q.tensor_columns < accumulator + 32 * q.ring) q.tensor_columns *= 2;
     const size_t share = kSharedPerSm * q.tensor_columns / kTensorColumns;
